@@ -13,6 +13,13 @@ from .real_pruning_fused_attention import (  # noqa: F401
     pack_flat_segments_kv,
     segmented_attention_plan,
 )
+from .paged_cache import (  # noqa: F401
+    PagedStep,
+    append_paged_kv,
+    build_paged_tables,
+    paged_shared_prefix_attention,
+    paged_window_attention,
+)
 from .slab_schedule import (  # noqa: F401
     SIDES_1M,
     SlabSchedule,

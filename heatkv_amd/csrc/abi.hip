@@ -10,6 +10,7 @@
 
 #include "../../include/heatkv.h"
 #include "hkv_internal.h"
+#include "paged.h"
 
 namespace {
 
@@ -730,6 +731,135 @@ int64_t hkv_segmented_attention_workspace_bytes(int32_t device) {
   if (need <= 0) return fail(HKV_ERR_DEVICE, "cannot query the CU count of device %d", device);
   ok();
   return need;
+}
+
+// ------------------------------------------------------------- paged cache
+
+namespace {
+
+// log2 of a block size, -1 when it is not a power of two in [1, 2^20]
+int32_t block_shift_of(int32_t block_size) {
+  for (int32_t s = 0; s <= 20; ++s)
+    if (block_size == 1 << s) return s;
+  return -1;
+}
+
+}  // namespace
+
+int32_t hkv_paged_tables(int32_t* block_tables, int64_t table_stride, const int32_t* lengths,
+                         const int32_t* new_counts, int32_t* free_blocks, const int32_t* free_range,
+                         int32_t requests, int32_t table_width, int32_t ring_size, int32_t num_tokens,
+                         int32_t block_size, int32_t window, int32_t sinks, int64_t* slot_map,
+                         int32_t* query_starts, int32_t* lengths_out, int32_t* range_out, int32_t* status,
+                         void* stream) {
+  const int32_t shift = block_shift_of(block_size);
+  if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
+  if (requests < 0 || table_width < 0 || ring_size < 0 || num_tokens < 0 || window < 0 || sinks < 0)
+    return fail(HKV_ERR_INVALID_ARG, "negative size, window or sinks");
+  if (requests > hkv::kMaxRequests)
+    return fail(HKV_ERR_UNSUPPORTED, "at most %d requests (got %d)", hkv::kMaxRequests, requests);
+  if (requests > 1 && table_stride < table_width)
+    return fail(HKV_ERR_INVALID_ARG, "table rows overlap (stride smaller than their width)");
+  if (!query_starts || !free_range || !range_out || !status || (num_tokens > 0 && !slot_map) ||
+      (ring_size > 0 && !free_blocks) ||
+      (requests > 0 && (!lengths || !new_counts || !lengths_out || (table_width > 0 && !block_tables))))
+    return fail(HKV_ERR_INVALID_ARG, "null pointer argument");
+  hkv::PagedTablesArgs a{block_tables, table_stride, lengths,     new_counts,   free_blocks, free_range, requests,
+                         table_width,  ring_size,    num_tokens,  shift,        window,      sinks,      slot_map,
+                         query_starts, lengths_out,  range_out,   status};
+  const hipError_t e = hkv::launch_paged_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(HKV_ERR_LAUNCH, "paged tables launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                         int64_t k_block_stride, int64_t k_cache_head_stride, int64_t k_row_stride,
+                         int64_t v_block_stride, int64_t v_cache_head_stride, int64_t v_row_stride,
+                         const int64_t* slot_map, int32_t num_blocks, int32_t num_tokens, int32_t kv_heads,
+                         int32_t head_dim, int32_t block_size, void* stream) {
+  const int32_t shift = block_shift_of(block_size);
+  if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
+  if (num_blocks < 0 || num_tokens < 0 || kv_heads <= 0)
+    return fail(HKV_ERR_INVALID_ARG, "negative size or no K/V heads");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes head_dim 64 or 128 (got %d)", head_dim);
+  if (num_tokens == 0 || num_blocks == 0) return ok();
+  if (!k || !v || !k_cache || !v_cache || !slot_map) return fail(HKV_ERR_INVALID_ARG, "null pointer argument");
+  hkv::PagedAppendArgs a{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, k_cache, v_cache,
+                         {k_block_stride, k_cache_head_stride, k_row_stride},
+                         {v_block_stride, v_cache_head_stride, v_row_stride},
+                         slot_map, static_cast<int64_t>(num_blocks) << shift, num_tokens, kv_heads, head_dim, shift};
+  const hipError_t e = hkv::launch_paged_append(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(HKV_ERR_LAUNCH, "paged append launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
+                                            int32_t head_dim, int32_t table_width, int32_t block_size,
+                                            int32_t prefix_length) {
+  (void)num_tokens; (void)requests; (void)heads; (void)kv_heads; (void)head_dim; (void)table_width;
+  (void)block_size; (void)prefix_length;
+  ok();
+  return 0;
+}
+
+int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                            const void* v_cache, int64_t k_block_stride, int64_t k_head_stride,
+                            int64_t k_row_stride, int64_t v_block_stride, int64_t v_head_stride,
+                            int64_t v_row_stride, const int32_t* block_tables, int64_t table_stride,
+                            const int32_t* lengths, const int32_t* query_starts, const int32_t* prefix_blocks,
+                            int32_t prefix_length, void* out, float* lse, int32_t num_tokens, int32_t requests,
+                            int32_t table_width, int32_t num_blocks, int32_t heads, int32_t kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t window, int32_t sinks, int32_t causal,
+                            int32_t dtype, float softmax_scale, int32_t fill_tail, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  const int32_t shift = block_shift_of(block_size);
+  if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
+  if (num_tokens < 0 || requests < 0 || table_width < 0 || num_blocks < 0 || window < 0 || sinks < 0 ||
+      prefix_length < 0)
+    return fail(HKV_ERR_INVALID_ARG, "negative size, window, sinks or prefix length");
+  if (requests > hkv::kMaxRequests)
+    return fail(HKV_ERR_UNSUPPORTED, "at most %d requests (got %d)", hkv::kMaxRequests, requests);
+  if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0)
+    return fail(HKV_ERR_INVALID_ARG, "heads must be a multiple of kv_heads (got %d, %d)", heads, kv_heads);
+  if (heads > 1024) return fail(HKV_ERR_UNSUPPORTED, "at most 1024 heads (got %d)", heads);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes head_dim 64 or 128 (got %d)", head_dim);
+  if (dtype != HKV_DTYPE_F16 && dtype != HKV_DTYPE_BF16)
+    return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes float16 or bfloat16 (got dtype code %d)", dtype);
+  if ((static_cast<int64_t>(table_width) << shift) > 0x7fffff00LL || prefix_length > 0x7fffff00)
+    return fail(HKV_ERR_UNSUPPORTED, "a table of more than 2^31 rows");
+  if (static_cast<int64_t>(num_tokens) * (heads / kv_heads) > 0x7fffff00LL)
+    return fail(HKV_ERR_UNSUPPORTED, "tokens times query heads per K/V head exceed 2^31");
+  if (num_tokens == 0) return ok();
+  if (!q || !out || !query_starts || (requests > 0 && (!lengths || (table_width > 0 && !block_tables))) ||
+      (prefix_length > 0 && !prefix_blocks))
+    return fail(HKV_ERR_INVALID_ARG, "null pointer argument");
+  if (num_blocks == 0 ? table_width > 0 || prefix_length > 0 : !k_cache || !v_cache)
+    return fail(HKV_ERR_INVALID_ARG, "no cache");
+  if (requests > 1 && table_stride < table_width)
+    return fail(HKV_ERR_INVALID_ARG, "table rows overlap (stride smaller than their width)");
+  const int64_t strides = q_token_stride | q_head_stride | k_block_stride | k_head_stride | k_row_stride |
+                          v_block_stride | v_head_stride | v_row_stride;
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
+                         reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out);
+  if (strides % 8 != 0 || ptrs % 16 != 0)
+    return fail(HKV_ERR_INVALID_ARG, "q, the caches and out must start at, and their rows lie, 16 bytes apart");
+  const int64_t need = hkv_paged_attention_workspace_bytes(num_tokens, requests, heads, kv_heads, head_dim,
+                                                           table_width, block_size, prefix_length);
+  if (need < 0) return static_cast<int32_t>(need);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256))
+    return fail(HKV_ERR_INVALID_ARG, "the call needs %lld bytes of 256-byte aligned workspace",
+                static_cast<long long>(need));
+  hkv::PagedAttnArgs a{q, q_token_stride, q_head_stride, k_cache, v_cache,
+                       {k_block_stride, k_head_stride, k_row_stride}, {v_block_stride, v_head_stride, v_row_stride},
+                       block_tables, table_stride, lengths, query_starts, prefix_blocks, prefix_length, out, lse,
+                       num_tokens, requests, table_width, num_blocks, heads, kv_heads, head_dim, shift, window, sinks,
+                       causal != 0 ? 1 : 0, dtype, fill_tail != 0 ? 1 : 0, softmax_scale, workspace, workspace_bytes};
+  const hipError_t e = hkv::launch_paged_attention(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(HKV_ERR_LAUNCH, "paged attention launch failed: %s", hipGetErrorString(e));
+  return ok();
 }
 
 }  // extern "C"

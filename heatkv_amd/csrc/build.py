@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 SOURCES = ("abi.hip", "pack.hip", "produce.hip", "plan.hip", "seg_attn.hip", "seg_attn_split.hip",
-           "seg_attn_staged.hip", "seg_attn_direct.hip")
+           "seg_attn_staged.hip", "seg_attn_direct.hip", "paged_tables.hip", "paged_attn.hip")
 ARCH = "gfx950"
 LIB = os.path.join(PKG, "libheatkv.so")
 

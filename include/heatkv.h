@@ -435,6 +435,79 @@ int32_t hkv_qkv_produce(const void* qkv, int64_t token_stride, const float* q_bi
                         int32_t head_dim, int32_t qkv_dtype, int32_t q_dtype, int32_t k_dtype,
                         int32_t v_dtype, int32_t normalize, float eps, void* stream);
 
+/*
+ * Paged K/V cache (no counterpart in the reference, whose cache holds one
+ * lockstep batch).  The cache holds rows of head_dim 16-bit elements in blocks
+ * of block_size rows (a power of two), addressed as
+ * cache[block * block_stride + head * head_stride + row * row_stride]
+ * (strides in elements); a request's block table names its blocks in order.
+ *
+ * hkv_paged_tables: the bookkeeping of one step on the GPU.  Request r holds
+ * lengths[r] rows and brings new_counts[r] tokens (< 0: it has ended).  The
+ * blocks it lacks are popped, in request order, from the head of the ring
+ * free_blocks[(first + i) % ring_size], i < count, free_range = (first, count),
+ * and entered in block_tables; blocks that no later token sees (all of an
+ * ended request's; with window > 0 those behind the first `sinks` rows' blocks
+ * that lie wholly before row lengths[r] + new_counts[r] - window + 1) are
+ * pushed behind the ring's tail in request and table order.  Popped are only blocks that were free
+ * before the step, so a pushed block may be read until the next step.
+ *   slot_map [num_tokens] : block * block_size + row of each token, in request
+ *       order; -1 behind the last
+ *   query_starts [requests + 1] : first token of each request
+ *   lengths_out, range_out : the state after the step (may be lengths, free_range)
+ *   status [1] : 0, or a sum of 1 (too few free blocks), 2 (a request does not
+ *       fit its table row), 4 (more tokens than num_tokens); then nothing is
+ *       popped, pushed or entered, the state is as before, every slot is -1 and every
+ *       query start 0.
+ */
+int32_t hkv_paged_tables(int32_t* block_tables, int64_t table_stride, const int32_t* lengths,
+                         const int32_t* new_counts, int32_t* free_blocks, const int32_t* free_range,
+                         int32_t requests, int32_t table_width, int32_t ring_size, int32_t num_tokens,
+                         int32_t block_size, int32_t window, int32_t sinks, int64_t* slot_map,
+                         int32_t* query_starts, int32_t* lengths_out, int32_t* range_out, int32_t* status,
+                         void* stream);
+
+/*
+ * K/V rows [num_tokens, kv_heads, head_dim] of a step's tokens to their slots
+ * (slots outside [0, num_blocks * block_size) are skipped; two tokens of one
+ * slot leave either's row).
+ */
+int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t v_token_stride, int64_t v_head_stride, void* k_cache, void* v_cache,
+                         int64_t k_block_stride, int64_t k_cache_head_stride, int64_t k_row_stride,
+                         int64_t v_block_stride, int64_t v_cache_head_stride, int64_t v_row_stride,
+                         const int64_t* slot_map, int32_t num_blocks, int32_t num_tokens, int32_t kv_heads,
+                         int32_t head_dim, int32_t block_size, void* stream);
+
+/*
+ * Attention over the paged cache.  Request r's queries are the tokens
+ * [query_starts[r], query_starts[r + 1]), the last of its lengths[r] rows:
+ * token i of n stands at row p = lengths[r] - n + i.  It sees row j of its
+ * request if j < lengths[r], j <= p (causal) and, with window > 0,
+ * j > p - window or j < sinks; and all prefix_length rows of the blocks
+ * prefix_blocks, which every request shares.  Query head h reads K/V head
+ * h / (heads / kv_heads).  out [num_tokens, heads * head_dim] of dtype;
+ * lse NULL or float32 [heads, num_tokens].  A query that sees nothing gets
+ * zeros and -inf; tokens behind the last request keep what they held
+ * (fill_tail 0) or get the same (fill_tail 1).  Table entries of rows that no
+ * query sees are not used.  workspace: hkv_paged_attention_workspace_bytes
+ * bytes (0: none needed), 256-byte aligned, contents before and after are of
+ * no meaning; calls that can overlap need buffers of their own.
+ */
+int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
+                                            int32_t head_dim, int32_t table_width, int32_t block_size,
+                                            int32_t prefix_length);
+int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                            const void* v_cache, int64_t k_block_stride, int64_t k_head_stride,
+                            int64_t k_row_stride, int64_t v_block_stride, int64_t v_head_stride,
+                            int64_t v_row_stride, const int32_t* block_tables, int64_t table_stride,
+                            const int32_t* lengths, const int32_t* query_starts, const int32_t* prefix_blocks,
+                            int32_t prefix_length, void* out, float* lse, int32_t num_tokens, int32_t requests,
+                            int32_t table_width, int32_t num_blocks, int32_t heads, int32_t kv_heads,
+                            int32_t head_dim, int32_t block_size, int32_t window, int32_t sinks, int32_t causal,
+                            int32_t dtype, float softmax_scale, int32_t fill_tail, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

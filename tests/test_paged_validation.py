@@ -1,0 +1,183 @@
+"""The paged cache's refusals (CPU tensors: shapes first, then the device), and its host oracle."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from heatkv_amd import (_lib, append_paged_kv, build_paged_tables, paged_shared_prefix_attention,
+                        paged_window_attention)
+from oracle import paged as opaged
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def _tables():
+    return dict(block_tables=i32(3, 8), lengths=i32(3), new_counts=i32(3), free_blocks=i32(20), free_range=i32(2),
+                num_tokens=4, block_size=16)
+
+
+def _append():
+    c = torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16)
+    return dict(k=torch.zeros((5, 2, 128), dtype=torch.bfloat16), v=torch.zeros((5, 2, 128), dtype=torch.bfloat16),
+                k_cache=c, v_cache=c.clone(), slot_map=torch.zeros(5, dtype=torch.int64))
+
+
+def _attn():
+    c = torch.zeros((6, 2, 16, 128), dtype=torch.bfloat16)
+    return dict(q=torch.zeros((5, 4, 128), dtype=torch.bfloat16), k_cache=c, v_cache=c.clone(), block_tables=i32(3, 8),
+                lengths=i32(3), query_starts=i32(4), softmax_scale=0.1)
+
+
+@pytest.mark.parametrize("change,error,msg", [
+    (dict(block_tables=i32(3)), ValueError, "block_tables"),
+    (dict(block_tables=torch.zeros((3, 8))), ValueError, "block_tables"),
+    (dict(block_tables=i32(8, 3).t()), ValueError, "contiguous rows"),
+    (dict(block_tables=i32(1, 8).expand(3, 8)), ValueError, "overlap"),
+    (dict(lengths=i32(4)), ValueError, "lengths"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int64)), ValueError, "lengths"),
+    (dict(new_counts=i32(6)[::2]), ValueError, "contiguous"),
+    (dict(free_blocks=i32(4, 5)), ValueError, "free_blocks"),
+    (dict(free_range=i32(3)), ValueError, "free_range"),
+    (dict(num_tokens=-1), ValueError, "num_tokens"),
+    (dict(block_size=12), ValueError, "power of two"),
+    (dict(block_size=0), ValueError, "power of two"),
+    (dict(window=-1), ValueError, "window"),
+    (dict(sinks=2**31), ValueError, "sinks"),
+    (dict(block_tables=i32(4097, 1), lengths=i32(4097), new_counts=i32(4097)), RuntimeError, "4096 requests"),
+    (dict(), RuntimeError, "requires CUDA tensors"),
+])
+def test_tables_refusals(change, error, msg):
+    with pytest.raises(error, match=msg):
+        build_paged_tables(**{**_tables(), **change})
+
+
+@pytest.mark.parametrize("change,error,msg", [
+    (dict(k=torch.zeros((5, 3, 128), dtype=torch.bfloat16)), ValueError, "k must be"),
+    (dict(v=torch.zeros((4, 2, 128), dtype=torch.bfloat16)), ValueError, "v must be"),
+    (dict(k=torch.zeros((5, 2, 128))), ValueError, "dtype"),
+    (dict(k=torch.zeros((5, 2, 256), dtype=torch.bfloat16)[..., ::2]), ValueError, "rows of k"),
+    (dict(k_cache=torch.zeros((6, 2, 16, 128))), ValueError, "dtype"),
+    (dict(v_cache=torch.zeros((7, 2, 16, 128), dtype=torch.bfloat16)), ValueError, "one shape"),
+    (dict(slot_map=torch.zeros(5, dtype=torch.int32)), ValueError, "slot_map"),
+    (dict(slot_map=torch.zeros(10, dtype=torch.int64)[::2]), ValueError, "slot_map"),
+    (dict(), RuntimeError, "requires CUDA tensors"),
+])
+def test_append_refusals(change, error, msg):
+    with pytest.raises(error, match=msg):
+        append_paged_kv(**{**_append(), **change})
+
+
+def test_cache_refusals():
+    for shape, dtype, error, msg in [((6, 2, 12, 128), torch.bfloat16, ValueError, "power of two"),
+                                     ((6, 2, 16, 96), torch.bfloat16, RuntimeError, "head_dim 64 or 128"),
+                                     ((6, 2, 16, 128), torch.float32, RuntimeError, "float16 or bfloat16"),
+                                     ((6, 0, 16, 128), torch.bfloat16, ValueError, "at least one K/V head"),
+                                     ((6, 2, 128), torch.bfloat16, ValueError, "num_blocks, kv_heads")]:
+        c = torch.zeros(shape, dtype=dtype)
+        with pytest.raises(error, match=msg):
+            paged_window_attention(**{**_attn(), "k_cache": c, "v_cache": c.clone()})
+
+
+@pytest.mark.parametrize("change,error,msg", [
+    (dict(q=torch.zeros((5, 4, 64), dtype=torch.bfloat16)), ValueError, "q must be"),
+    (dict(q=torch.zeros((5, 4, 128), dtype=torch.float16)), ValueError, "dtype"),
+    (dict(q=torch.zeros((5, 3, 128), dtype=torch.bfloat16)), ValueError, "multiple"),
+    (dict(q=torch.zeros((5, 0, 128), dtype=torch.bfloat16)), ValueError, "multiple"),
+    (dict(q=torch.zeros((1, 1026, 128), dtype=torch.bfloat16)), RuntimeError, "1024 heads"),
+    (dict(query_starts=i32(3)), ValueError, "query_starts"),
+    (dict(lengths=i32(2)), ValueError, "lengths"),
+    (dict(window=-5), ValueError, "window"),
+    (dict(out=torch.zeros((5, 512))), ValueError, "out must be"),
+    (dict(out=torch.zeros((5, 1024), dtype=torch.bfloat16)[:, ::2]), ValueError, "contiguous"),
+    (dict(), RuntimeError, "requires CUDA tensors"),
+])
+def test_attention_refusals(change, error, msg):
+    with pytest.raises(error, match=msg):
+        paged_window_attention(**{**_attn(), **change})
+
+
+@pytest.mark.parametrize("change,error,msg", [
+    (dict(prefix_blocks=None), ValueError, "prefix_blocks"),
+    (dict(prefix_blocks=i32(2, 2)), ValueError, "prefix_blocks"),
+    (dict(prefix_length=65), ValueError, "prefix_blocks hold 64 rows"),
+    (dict(prefix_length=-1), ValueError, "prefix_length"),
+    (dict(), RuntimeError, "requires CUDA tensors"),
+])
+def test_prefix_refusals(change, error, msg):
+    a = {**_attn(), "prefix_blocks": i32(4), "prefix_length": 60, **change}
+    with pytest.raises(error, match=msg):
+        paged_shared_prefix_attention(**a)
+
+
+def test_abi_refusals_before_any_device_call():
+    """The library's own checks, for callers of the C ABI."""
+    lib = _lib.load()
+    n = None
+    tables = lambda *v: lib.hkv_paged_tables(n, 8, n, n, n, n, *v, n, n, n, n, n, n)  # noqa: E731
+    assert tables(1, 8, 4, 1, 12, 0, 0) == _lib.HKV_ERR_INVALID_ARG and "power of two" in _lib.last_error()
+    assert tables(5000, 8, 4, 1, 16, 0, 0) == _lib.HKV_ERR_UNSUPPORTED
+    assert tables(1, -8, 4, 1, 16, 0, 0) == _lib.HKV_ERR_INVALID_ARG
+    assert tables(1, 8, 4, 1, 16, 0, 0) == _lib.HKV_ERR_INVALID_ARG and "null" in _lib.last_error()
+    append = lambda *v: lib.hkv_paged_append(n, n, 0, 0, 0, 0, n, n, 0, 0, 0, 0, 0, 0, n, *v, n)  # noqa: E731
+    assert append(4, 1, 2, 96, 16) == _lib.HKV_ERR_UNSUPPORTED
+    assert append(4, 1, 2, 128, 16) == _lib.HKV_ERR_INVALID_ARG
+    assert append(4, 0, 2, 128, 16) == 0
+
+    def attn(T=1, R=1, M=4, N=4, H=4, hk=2, D=128, block=16, dtype=2, strides=128, prefix=0):
+        import ctypes
+        return lib.hkv_paged_attention(n, strides, strides, n, n, strides, strides, strides, strides, strides, strides,
+                                       n, M, n, n, n, prefix, n, n, T, R, M, N, H, hk, D, block, 0, 0, 1, dtype,
+                                       ctypes.c_float(1.0), 1, n, 0, n)
+    assert attn(H=3) == _lib.HKV_ERR_INVALID_ARG
+    assert attn(D=96) == _lib.HKV_ERR_UNSUPPORTED
+    assert attn(dtype=3) == _lib.HKV_ERR_UNSUPPORTED
+    assert attn(block=24) == _lib.HKV_ERR_INVALID_ARG
+    assert attn(M=2**27) == _lib.HKV_ERR_UNSUPPORTED
+    assert attn(R=5000) == _lib.HKV_ERR_UNSUPPORTED
+    assert attn(T=2**30, H=8, hk=1) == _lib.HKV_ERR_UNSUPPORTED
+    assert attn() == _lib.HKV_ERR_INVALID_ARG
+    assert attn(T=0) == 0
+
+
+def test_oracle_tables_keep_every_block_once():
+    """The free list and the live blocks of the requests partition the blocks, whatever the steps."""
+    rng = np.random.default_rng(0)
+    for window, sinks, block in [(0, 0, 4), (9, 0, 4), (9, 5, 4), (1, 0, 1), (30, 64, 16)]:
+        N = 400 // block
+        tables, lengths = np.full((5, 200 // block + 1), -1), np.zeros(5, np.int32)
+        ring, span = rng.permutation(N).astype(np.int32), np.array([0, N], np.int32)
+        for _ in range(60):
+            counts = np.where((lengths > 90) | (rng.random(5) < 0.1), -1, rng.integers(0, 8, 5))
+            tables, ring, slots, starts, lengths, span, status = opaged.build_tables(
+                tables, lengths, counts, ring, span, 40, block, window, sinks)
+            assert status == 0 and starts[-1] == (slots >= 0).sum() == np.maximum(counts, 0).sum()
+            free = [int(ring[(span[0] + i) % N]) for i in range(span[1])]
+            live = []
+            for r in range(5):
+                for j in range(-(-int(lengths[r]) // block)):
+                    seen = window == 0 or j < -(-sinks // block) or (j + 1) * block > lengths[r] - window + 1
+                    if seen:
+                        live.append(int(tables[r, j]))
+            assert sorted(free + live) == list(range(N))
+
+
+def test_oracle_attention_against_torch():
+    """On one request without holes the oracle is torch's softmax attention in 64 bits."""
+    gen = torch.Generator().manual_seed(0)
+    K = torch.randn((3, 2, 8, 64), generator=gen, dtype=torch.float64)
+    V = torch.randn((3, 2, 8, 64), generator=gen, dtype=torch.float64)
+    q = torch.randn((20, 4, 64), generator=gen, dtype=torch.float64)
+    out, lse, tol, _ = opaged.attention(q.numpy(), K.numpy(), V.numpy(), np.array([[2, 0, 1]]), [20], [0, 20], 0.3,
+                                        2.0**-8)
+    order = [2, 0, 1]
+    k = K[order].transpose(0, 1).reshape(2, 24, 64)[:, :20].repeat_interleave(2, 0)
+    v = V[order].transpose(0, 1).reshape(2, 24, 64)[:, :20].repeat_interleave(2, 0)
+    s = (q.transpose(0, 1) @ k.transpose(1, 2) * 0.3).masked_fill(torch.ones(20, 20).triu(1).bool(), -float("inf"))
+    want = (s.softmax(-1) @ v).transpose(0, 1).numpy()
+    np.testing.assert_allclose(out, want, atol=1e-12)
+    np.testing.assert_allclose(lse, s.logsumexp(-1).numpy(), atol=1e-12)
+    assert (tol > 0).all()
