@@ -798,10 +798,15 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
                                             int32_t prefix_length) {
-  (void)num_tokens; (void)requests; (void)heads; (void)kv_heads; (void)head_dim; (void)table_width;
-  (void)block_size; (void)prefix_length;
+  const int32_t shift = block_shift_of(block_size);
+  if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
+  if (num_tokens < 0 || requests < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || table_width < 0 ||
+      prefix_length < 0)
+    return fail(HKV_ERR_INVALID_ARG, "negative size, or heads no multiple of kv_heads");
   ok();
-  return 0;
+  return num_tokens == 0 ? 0
+                         : hkv::paged_attention_workspace(num_tokens, requests, heads, kv_heads, head_dim,
+                                                          static_cast<int64_t>(table_width) << shift, prefix_length);
 }
 
 int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,

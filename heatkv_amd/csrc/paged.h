@@ -86,5 +86,7 @@ struct PagedAttnArgs {
   int64_t workspace_bytes;
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                  int64_t table_rows, int32_t prefix_len);
 
 }  // namespace hkv

@@ -2,8 +2,22 @@
 // its request's blocks (with a causal limit, a sliding window and first rows
 // that stay visible), and of a prefix that all requests share.
 //
-// One wave per (token, query head): 64 keys at a time, a key per lane for the
-// scores, two dimensions per lane for the values.
+// The queries of one request and K/V head are a matrix of n * group rows (token
+// by token, the heads of a group side by side) against one stream of keys.  Two
+// kernels run tiles of those rows:
+//  * paged_wide_kernel, 128 rows, matrix-bound: prompts and scales.
+//  * paged_narrow_kernel, 16 rows, bound by the bytes of the cache: single tokens.
+//
+// Plan.  Nothing about the requests is known on the host, so every workgroup
+// finds its work from lengths and query_starts itself: tiles of rows per
+// request, 64-key chunks per tile, and, so that few rows over long keys still
+// fill the card, `parts` of a tile's chunks.  With `total` chunks in the launch
+// a part has c = max(least, total / units wanted) of them, so there are at most
+// tiles + wanted units per K/V head (the grid) and 2 * wanted of them belong
+// to tiles that are cut (their partial results' records).  A tile that is not
+// cut writes its output; the parts of the others leave an unnormalized O, a
+// maximum and a sum, which paged_combine_kernel joins in part order, so results do
+// not depend on the order of arrival and nothing has to be cleared or waited for.
 #include "attn_common.h"
 #include "paged.h"
 
@@ -12,107 +26,855 @@ namespace {
 
 using namespace attn;
 
-template <int DT>
-__device__ __forceinline__ float widen(uint16_t v) {
-  if constexpr (DT == kF16) return f16_to_f32(v);
-  else return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16);
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_ptr;
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+
+constexpr int kWideRows = 128;
+constexpr float kNoMax = -1e30f;
+
+// ---------------------------------------------------------------- plan
+
+// One launch: the requests' own rows, or (shared) the prefix for the rows of
+// all requests together.
+struct PagedPass {
+  int32_t shared;    // one pseudo request: all live tokens, the prefix's keys
+  int32_t with_prefix;  // each tile's keys begin with the prefix (wide tiles that need no sharing)
+  int32_t rows;      // rows of a tile
+  int32_t least;     // chunks of a part at least
+  int32_t wanted;    // units per K/V head that fill the card
+  int32_t always;    // every tile leaves records (a shared prefix is joined to it)
+  int32_t combined;  // a combine launch follows: write meta
+  float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
+  int2* meta;        // per live row: first record, parts | row in tile << 16
+};
+
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+struct Geometry {
+  int32_t n;      // queries
+  int32_t first;  // token of query 0
+  int32_t len;    // rows
+};
+
+__device__ __forceinline__ int32_t clamp32(int32_t v, int32_t lo, int32_t hi) {
+  return v < lo ? lo : (v > hi ? hi : v);
 }
 
-template <int DT>
-__device__ __forceinline__ uint16_t narrow(float v) {
-  return static_cast<uint16_t>(pack2<DT>(v, v) & 0xffffu);
+__device__ __forceinline__ int32_t live_tokens(const PagedAttnArgs& a) {
+  return a.requests > 0 ? clamp32(a.query_starts[a.requests], 0, a.num_tokens) : 0;
 }
 
+__device__ __forceinline__ Geometry load_request(const PagedAttnArgs& a, const PagedPass& p, int32_t r) {
+  Geometry g;
+  if (p.shared) {
+    g.first = 0;
+    g.n = live_tokens(a);
+    g.len = a.prefix_len;
+    return g;
+  }
+  g.first = clamp32(a.query_starts[r], 0, a.num_tokens);
+  g.n = clamp32(a.query_starts[r + 1], g.first, a.num_tokens) - g.first;
+  g.len = clamp32(a.lengths[r], 0, a.table_width << a.block_shift);
+  return g;
+}
+
+// The keys that queries [i0, i1] of a request see: rows [0, sinks) and
+// [lo, hi), as chunks [0, na) and [b0, b0 + nb) behind the prefix's np.
+struct Keys {
+  int32_t lo, hi, sinks;
+  int32_t np, na, b0, nb;
+  __device__ __forceinline__ int32_t chunks() const { return np + na + nb; }
+};
+
+__device__ __forceinline__ Keys keys_of(const PagedAttnArgs& a, const PagedPass& p, const Geometry& g, int32_t i0,
+                                        int32_t i1) {
+  Keys k{0, 0, 0, 0, 0, 0, 0};
+  if (p.shared) {
+    k.hi = g.len;
+  } else {
+    const int32_t p0 = g.len - g.n + i0, p1 = g.len - g.n + i1;
+    k.hi = p1 < 0 ? 0 : (a.causal ? p1 + 1 : g.len);
+    if (a.window > 0 && p0 >= a.window) {
+      k.lo = p0 - a.window + 1;
+      k.sinks = a.sinks < k.hi ? a.sinks : k.hi;
+      if (k.lo <= k.sinks) k.lo = k.sinks = 0;
+    }
+    if (p.with_prefix) k.np = (a.prefix_len + kBN - 1) / kBN;
+  }
+  if (k.hi > 0) {
+    k.na = (k.sinks + kBN - 1) / kBN;
+    k.b0 = k.lo / kBN > k.na ? k.lo / kBN : k.na;
+    k.nb = (k.hi + kBN - 1) / kBN - k.b0;
+    if (k.nb < 0) k.nb = 0;
+  }
+  return k;
+}
+
+struct Load {
+  int32_t tiles, chunks;  // of a request: tiles of rows, chunks of the longest tile
+};
+
+__device__ __forceinline__ Load load_of(const PagedAttnArgs& a, const PagedPass& p, const Geometry& g) {
+  const int32_t group = a.heads / a.kv_heads;
+  Load l{0, 0};
+  if (g.n == 0) return l;
+  l.tiles = (g.n * group + p.rows - 1) / p.rows;
+  l.chunks = keys_of(a, p, g, 0, g.n - 1).chunks();
+  return l;
+}
+
+struct Work {
+  int32_t request;  // -1: none
+  int32_t tile;
+  int32_t part;
+  int32_t parts;    // of the request's tiles
+  int32_t record;   // of the tile's part 0
+};
+
+__device__ __forceinline__ int32_t parts_of(const Load& l, int64_t c) {
+  return l.chunks > c ? static_cast<int32_t>((l.chunks + c - 1) / c) : 1;
+}
+
+// Units, and records, of a request.
+__device__ __forceinline__ int2 units_of(const PagedPass& p, const Load& l, int64_t c) {
+  const int32_t parts = parts_of(l, c);
+  const int32_t units = l.tiles * parts;
+  return int2{units, parts > 1 || p.always ? units : 0};
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+__device__ __forceinline__ int2 wave_prefix(int2 v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int2 o{__shfl_up(v.x, off, 64), __shfl_up(v.y, off, 64)};
+    if (lane >= off) v = int2{v.x + o.x, v.y + o.y};
+  }
+  return v;
+}
+
+// Work of unit `unit` (per K/V head).  Up to 64 requests every wave plans by
+// itself, a request per lane; more are dealt to the workgroup's threads in runs.
+template <int kThreads>
+__device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
+  const int32_t R = p.shared ? 1 : a.requests;
+  const int lane = threadIdx.x & 63;
+  Work w{-1, 0, 0, 1, 0};
+  if (R <= 64) {
+    Load l{0, 0};
+    if (lane < R) l = load_of(a, p, load_request(a, p, lane));
+    const int64_t total = wave_sum64(static_cast<int64_t>(l.tiles) * l.chunks);
+    int64_t c = (total + p.wanted - 1) / p.wanted;
+    c = c < p.least ? p.least : c;
+    const int2 mine = units_of(p, l, c);
+    const int2 end = wave_prefix(mine);
+    const uint64_t hit = __ballot(unit >= end.x - mine.x && unit < end.x);
+    if (hit == 0) return w;
+    const int src = __builtin_ctzll(hit);
+    const int32_t parts = __builtin_amdgcn_readlane(parts_of(l, c), src);
+    const int32_t in = uniform(unit - __builtin_amdgcn_readlane(end.x - mine.x, src));
+    w.request = src;
+    w.parts = parts;
+    w.part = in % parts;
+    w.tile = __builtin_amdgcn_readlane(l.tiles, src) - 1 - in / parts;  // causal tiles: longest first
+    w.record = __builtin_amdgcn_readlane(end.y - mine.y, src) + w.tile * parts;
+    return w;
+  }
+  constexpr int kWaves = kThreads / 64;
+  __shared__ int64_t wave_total[kWaves];
+  __shared__ int2 wave_units[kWaves];
+  __shared__ int32_t found[5];
+  const int tid = threadIdx.x;
+  const int wave = tid >> 6;
+  const int32_t run = (R + kThreads - 1) / kThreads;
+  const int32_t r0 = tid * run < R ? tid * run : R, r1 = r0 + run < R ? r0 + run : R;
+  int64_t sum = 0;
+  for (int32_t r = r0; r < r1; ++r) {
+    const Load l = load_of(a, p, load_request(a, p, r));
+    sum += static_cast<int64_t>(l.tiles) * l.chunks;
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) wave_total[wave] = sum;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  int64_t total = 0;
+  for (int i = 0; i < kWaves; ++i) total += wave_total[i];
+  int64_t c = (total + p.wanted - 1) / p.wanted;
+  c = c < p.least ? p.least : c;
+  int2 mine{0, 0};
+  for (int32_t r = r0; r < r1; ++r) {
+    const int2 u = units_of(p, load_of(a, p, load_request(a, p, r)), c);
+    mine = int2{mine.x + u.x, mine.y + u.y};
+  }
+  int2 end = wave_prefix(mine);
+  if (lane == 63) wave_units[wave] = end;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) end = int2{end.x + wave_units[i].x, end.y + wave_units[i].y};
+  int2 at{end.x - mine.x, end.y - mine.y};
+  if (unit >= at.x && unit < end.x) {  // one thread
+    for (int32_t r = r0; r < r1; ++r) {
+      const Load l = load_of(a, p, load_request(a, p, r));
+      const int2 u = units_of(p, l, c);
+      if (unit < at.x + u.x) {
+        const int32_t parts = parts_of(l, c);
+        const int32_t in = unit - at.x;
+        found[0] = r;
+        found[1] = l.tiles - 1 - in / parts;
+        found[2] = in % parts;
+        found[3] = parts;
+        found[4] = at.y + found[1] * parts;
+        break;
+      }
+      at = int2{at.x + u.x, at.y + u.y};
+    }
+  }
+  __syncthreads();
+  w.request = __builtin_amdgcn_readfirstlane(found[0]);
+  if (w.request < 0) return w;
+  w.tile = __builtin_amdgcn_readfirstlane(found[1]);
+  w.part = __builtin_amdgcn_readfirstlane(found[2]);
+  w.parts = __builtin_amdgcn_readfirstlane(found[3]);
+  w.record = __builtin_amdgcn_readfirstlane(found[4]);
+  return w;
+}
+
+// ---------------------------------------------------------------- a tile of rows
+
+struct Tile {
+  Geometry g;
+  Keys keys;
+  const int32_t* blocks;  // of the request's own keys (shared: the prefix's)
+  int32_t row0, rows;     // rows of the request's matrix
+  int32_t t0, t1;         // chunks of this part
+  int32_t parts;          // of this tile
+  int32_t one;            // all rows stand at one position
+};
+
+// Whether there is work; part and tile of `w` as its tile cuts them.
+__device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPass& p, const Work& w, Tile& t) {
+  const int32_t group = a.heads / a.kv_heads;
+  t.g = load_request(a, p, w.request);
+  t.g.n = uniform(t.g.n);
+  t.g.first = uniform(t.g.first);
+  t.g.len = uniform(t.g.len);
+  t.row0 = w.tile * p.rows;
+  t.rows = t.g.n * group - t.row0;
+  t.rows = t.rows < p.rows ? t.rows : p.rows;
+  const int32_t i0 = t.row0 / group, i1 = (t.row0 + t.rows - 1) / group;
+  t.one = i0 == i1;
+  t.keys = keys_of(a, p, t.g, i0, i1);
+  t.blocks = p.shared ? a.prefix_blocks : a.block_tables + w.request * a.table_stride;
+  const int32_t n = t.keys.chunks();
+  // a tile with fewer chunks than its request's longest is cut in fewer parts
+  const int32_t most = (n + p.least - 1) / p.least;
+  t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
+  if (w.part >= t.parts) return false;
+  t.t0 = static_cast<int32_t>(static_cast<int64_t>(n) * w.part / t.parts);
+  t.t1 = static_cast<int32_t>(static_cast<int64_t>(n) * (w.part + 1) / t.parts);
+  return true;
+}
+
+// First row of the part's t-th chunk, and whether it is the prefix's.
+__device__ __forceinline__ int32_t chunk_row(const Keys& k, int32_t t, bool& prefix) {
+  prefix = t < k.np;
+  if (prefix) return t * kBN;
+  t -= k.np;
+  return (t < k.na ? t : t - k.na + k.b0) * kBN;
+}
+
+// The row to load for row j of a chunk: rows that no query of the tile sees
+// (past the end, or between the sinks and the window) stand for one that is
+// seen, so that their weight of 0 meets no stray NaN and no stale table entry.
+__device__ __forceinline__ int32_t row_to_load(const PagedAttnArgs& a, const Keys& k, int32_t j, bool prefix) {
+  if (prefix) return j < a.prefix_len ? j : a.prefix_len - 1;
+  if (j >= k.hi) return k.hi - 1;
+  if (j < k.lo && j >= k.sinks) return (j & ~(kBN - 1)) < k.sinks ? k.sinks - 1 : k.lo;
+  return j;
+}
+
+__device__ __forceinline__ int64_t block_of(const PagedAttnArgs& a, int32_t raw) {
+  return static_cast<uint32_t>(raw) < static_cast<uint32_t>(a.num_blocks) ? raw : 0;
+}
+
+// What a query (row of the matrix) sees of its request's own rows.
+struct Sight {
+  int32_t lo, hi;
+};
+
+__device__ __forceinline__ Sight sight_of(const PagedAttnArgs& a, const PagedPass& p, const Geometry& g, int32_t i) {
+  Sight s{0, g.len};
+  if (!p.shared) {
+    const int32_t pos = g.len - g.n + i;
+    if (pos < 0) s.hi = 0;
+    else if (a.causal) s.hi = pos + 1;
+    if (a.window > 0) s.lo = pos - a.window + 1;
+  }
+  return s;
+}
+
+// Whether each query of the tile sees each row of the 64 (or `n`) from j.
+__device__ __forceinline__ bool all_seen(const PagedAttnArgs& a, const Sight& first, const Sight& last, int32_t j,
+                                         bool prefix, int32_t n = kBN) {
+  if (prefix) return j + n <= a.prefix_len;
+  return j + n <= first.hi && (j >= last.lo || j + n <= a.sinks);
+}
+
+// 16 bytes per lane from `src` straight to LDS at lds + 16 lane (uniform lds).
+// Inline assembly, so that the compiler, which cannot see the LDS write, does not
+// make LDS reads wait for every load: the kernels wait themselves.  M0 is
+// written here and nothing else in these kernels uses it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_ptr)(p)));
+}
+
+__device__ __forceinline__ u32x2_t ds_read_tr(const uint8_t* p) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p)));
+}
+
+// Takes the values that are not finite out of an operand: 1 in `up` for +inf and
+// NaN, in `down` for -inf and NaN.
+template <int DT>
+__device__ __forceinline__ void split_finite(u32x4_t& v, u32x4_t& up, u32x4_t& down) {
+  constexpr uint32_t kExp = DT == kF16 ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kOne = DT == kF16 ? 0x3c00u : 0x3f80u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x[2] = {v[i] & 0xffffu, v[i] >> 16};
+    uint32_t keep[2], hi[2], lo[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bool odd = (x[k] & kExp) == kExp;
+      const bool nan = odd && (x[k] & 0x7fffu) != kExp;
+      keep[k] = odd ? 0u : x[k];
+      hi[k] = odd && (nan || x[k] < 0x8000u) ? kOne : 0u;
+      lo[k] = odd && (nan || x[k] >= 0x8000u) ? kOne : 0u;
+    }
+    v[i] = keep[0] | keep[1] << 16;
+    up[i] = hi[0] | hi[1] << 16;
+    down[i] = lo[0] | lo[1] << 16;
+  }
+}
+
+// Zeros (lse -inf) for the tokens behind the last request, shared by all workgroups.
+template <int kThreads>
+__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a) {
+  const int32_t live = live_tokens(a);
+  if (live >= a.num_tokens) return;
+  const int64_t units = static_cast<int64_t>(a.num_tokens - live) * a.heads * (a.head_dim / 8);
+  uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
+                                              static_cast<int64_t>(live) * a.heads * a.head_dim);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t i = at; i < units; i += step) out[i] = uint4{0, 0, 0, 0};
+  if (a.lse == nullptr) return;
+  const int32_t tail = a.num_tokens - live;
+  for (int64_t i = at; i < static_cast<int64_t>(tail) * a.heads; i += step)
+    a.lse[(i / tail) * a.num_tokens + live + i % tail] = -__builtin_inff();
+}
+
+// Record of (part of a tile, K/V head).
+template <int D>
+__device__ __forceinline__ float* record_of(const PagedAttnArgs& a, const PagedPass& p, int32_t record, int32_t kvh) {
+  return p.records + (static_cast<int64_t>(record) * a.kv_heads + kvh) * (p.rows * (D + 2));
+}
+
+template <int kThreads>
+__device__ __forceinline__ void write_meta(const PagedAttnArgs& a, const PagedPass& p, const Tile& t, const Work& w,
+                                           int32_t kvh) {
+  if (!p.combined || w.part != 0 || kvh != 0) return;
+  const int32_t group = a.heads / a.kv_heads;
+  for (int32_t i = threadIdx.x; i < t.rows; i += kThreads)
+    p.meta[static_cast<int64_t>(t.g.first) * group + t.row0 + i] = int2{w.record, t.parts | i << 16};
+}
+
+// ---------------------------------------------------------------- wide tiles
+//
+// Four waves of 32 rows; per 64-key chunk S^T = K Q^T and O^T += V^T P^T on the
+// 32x32x16 MFMAs, softmax in the exp2 domain with a lazily moved maximum, as
+// the segmented kernel (seg_attn_direct.hip, whose operand order in LDS this
+// one shares): chunks go straight to LDS, two stages, K one chunk ahead of V, so
+// iteration t runs S(t + 1) on the matrix cores beside the exponentials of S(t).
+// Waves 0 and 1 load the K rows, 2 and 3 the V rows, each lane the rows of its
+// own; the table entries of the next chunk are read one iteration ahead.
 template <int DT, int D>
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedAttnArgs a) {
-  constexpr int kPer = D / 64;
-  __shared__ float qs[D];
-  const int lane = threadIdx.x;
-  const int32_t t = static_cast<int32_t>(blockIdx.x);
-  const int32_t h = static_cast<int32_t>(blockIdx.y);
-  const int32_t kvh = h / (a.heads / a.kv_heads);
-  const int32_t R = a.requests;
-  uint16_t* const out = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(t) * a.heads + h) * D;
-  // the request of the token: the last one that starts at or before it
-  const int32_t end = R > 0 ? a.query_starts[R] : 0;
-  if (t >= end) {
-    if (a.fill_tail) {
-      for (int i = 0; i < kPer; ++i) out[lane * kPer + i] = 0;
-      if (a.lse != nullptr && lane == 0) a.lse[static_cast<int64_t>(h) * a.num_tokens + t] = -__builtin_inff();
+__global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                            const Scalars sc) {
+  constexpr int kThreads = 256;
+  constexpr int KS = D / 16;               // k-steps of S
+  constexpr int DB = D / 32;               // 32-wide blocks of O
+  constexpr int NP = D / 64;               // V DMAs per 8 rows
+  constexpr int kTensor = kBN * D * 2;     // bytes of a chunk's K or V
+  constexpr int kStage = 2 * kTensor;
+  constexpr int kPitch = D * 2 + 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kStage < 4 * 32 * kPitch ? 4 * 32 * kPitch : 2 * kStage];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5;
+  const int32_t group = a.heads / a.kv_heads;
+  const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
+  if (a.fill_tail && !p.shared) fill_tail<kThreads>(a);
+  const Work w = find_work<kThreads>(a, p, unit);
+  Tile t;
+  if (w.request < 0 || !make_tile(a, p, w, t)) return;
+  write_meta<kThreads>(a, p, t, w, kvh);
+
+  // this lane's row (rows past the tile's last repeat it and are not stored)
+  const int32_t row = wave * 32 + (lane & 31);
+  const int32_t mat = t.row0 + (row < t.rows ? row : t.rows - 1);
+  const int32_t tok = mat / group;
+  const Sight mine = sight_of(a, p, t.g, tok);
+  const Sight first = sight_of(a, p, t.g, t.row0 / group);
+  const Sight last = sight_of(a, p, t.g, (t.row0 + t.rows - 1) / group);
+  u32x4_t qf[KS];
+  {
+    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (t.g.first + tok) * a.q_token +
+                              (kvh * group + (mat - tok * group)) * a.q_head + g * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4_t*>(q + ks * 16);
+  }
+
+  f32x16_t oacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) oacc[i] = f32x16_t{};
+  float m_run = kNoMax, l_run = 0.f;
+
+  if (t.t0 < t.t1) {
+    // Rows of this wave in a chunk: [32 half, + 32).  K lanes hold one row (key
+    // lane % 32), V lanes four (key 8 i + 4 (lp / 16) + (lp % 8) / 2).
+    const bool k_wave = wave < 2;
+    const int half = wave & 1;
+    const int lp = lane & 31;
+    const int key0 = 32 * half + (k_wave ? lp : 4 * (lp >> 4) + ((lp & 7) >> 1));
+    const int col = k_wave ? 16 * g : 2 * (32 * g + 16 * ((lp >> 3) & 1) + 8 * (lp & 1));
+    const PagedCacheStrides cs = k_wave ? a.ks : a.vs;
+    const uint8_t* const cache =
+        static_cast<const uint8_t*>(k_wave ? a.k_cache : a.v_cache) + kvh * cs.head * 2 + col;
+    const uint32_t lds = lds_address(ring) + (k_wave ? half * (KS * 1024) : kTensor + half * (4 * NP * 1024));
+    const int32_t mask = (1 << a.block_shift) - 1;
+    int32_t rows[4], ids[4];
+    // table entries of the chunk at stream position c
+    auto look_up = [&](int32_t c) {
+      bool prefix;
+      const int32_t j0 = chunk_row(t.keys, c, prefix) + key0;
+      const int32_t* const blocks = prefix ? a.prefix_blocks : t.blocks;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i > 0 && k_wave) break;
+        rows[i] = row_to_load(a, t.keys, j0 + 8 * i, prefix);
+        ids[i] = blocks[rows[i] >> a.block_shift];
+      }
+    };
+    auto pointer = [&](int i) {
+      return cache + (block_of(a, ids[i]) * cs.block + static_cast<int64_t>(rows[i] & mask) * cs.row) * 2;
+    };
+    // the chunk whose entries were looked up, into stage c % 2
+    auto issue = [&](int32_t c) {
+      const uint32_t dst = lds + (c & 1) * kStage;
+      if (k_wave) {
+        const uint8_t* const src = pointer(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) dma16(src + 32 * ks, dst + 1024 * ks);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* const src = pointer(i);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) dma16(src + 128 * n, dst + 1024 * (i * NP + n));
+        }
+      }
+    };
+
+    auto qk = [&](f32x16_t (&sx)[2], int32_t c) {
+      const uint8_t* const kst = ring + (c & 1) * kStage + lane * 16;
+      sx[0] = f32x16_t{};
+      sx[1] = f32x16_t{};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          sx[kb] = mfma32<DT>(*reinterpret_cast<const u32x4_t*>(kst + (kb * KS + ks) * 1024), qf[ks], sx[kb]);
+    };
+    auto v_operand = [&](const uint8_t* vst, int u, int db) {
+      const uint8_t* const at = vst + (u * 2 * NP + (db >> 1)) * 1024 + (db & 1) * 512;
+      const u32x2_t lo = ds_read_tr(at), hi = ds_read_tr(at + NP * 1024);
+      return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto pv = [&](const u32x4_t (&pf)[4], int32_t c) {
+      const uint8_t* const vst = ring + (c & 1) * kStage + kTensor + lane * 8;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) oacc[db] = mfma32<DT>(v_operand(vst, u, db), pf[u], oacc[db]);
+    };
+    // Rows of chunk c that this lane's query does not see: score -inf.
+    auto hide = [&](f32x16_t (&sx)[2], int32_t j0, bool prefix) {
+      const int32_t hi = (prefix ? a.prefix_len : mine.hi) - j0 - 4 * g;
+      const int32_t lo = (prefix ? 0 : mine.lo) - j0 - 4 * g;
+      const int32_t sinks = a.sinks - j0 - 4 * g;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int32_t j = kb * 32 + 8 * (i >> 2) + (i & 3);
+          sx[kb][i] = (j >= hi) | ((j < lo) & (j >= sinks)) ? -__builtin_inff() : sx[kb][i];
+        }
+    };
+    auto pack = [&](const f32x16_t (&sx)[2], u32x4_t (&pf)[4]) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) pf[u] = p_operand<DT>(sx, u);
+    };
+    auto move = [&](float mx) {
+      if (__any(mx - m_run > sc.thresh)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * sc.c);
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
+        m_run = m_new;
+      }
+    };
+    auto hidden = [&](int32_t c, int32_t& j0, bool& prefix) {
+      j0 = chunk_row(t.keys, c, prefix);
+      return !all_seen(a, first, last, j0, prefix);
+    };
+
+    // Prologue: chunk t0 whole, K(t0 + 1) in flight; V waves look up t0 + 1, K waves t0 + 2.
+    look_up(t.t0);
+    issue(t.t0);
+    if (t.t0 + 1 < t.t1) look_up(t.t0 + 1);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] ^= sc.q_sign;
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (k_wave && t.t0 + 1 < t.t1) {
+      issue(t.t0 + 1);
+      if (t.t0 + 2 < t.t1) look_up(t.t0 + 2);
+    }
+    f32x16_t sa[2], sb[2];
+    int32_t j0;
+    bool prefix;
+    qk(sa, t.t0);
+    if (hidden(t.t0, j0, prefix)) hide(sa, j0, prefix);
+    move(tile_max(sa));
+
+    auto weigh = [&](f32x16_t (&s)[2], int32_t c) {
+      u32x4_t pf[4];
+      exp_tile(s, m_run, sc.c, l_run);
+      pack(s, pf);
+      pv(pf, c);
+    };
+    auto step = [&](f32x16_t (&cur)[2], f32x16_t (&next)[2], int32_t c) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      const int32_t ahead = c + (k_wave ? 2 : 1);
+      if (ahead < t.t1) {
+        issue(ahead);
+        if (ahead + 1 < t.t1) look_up(ahead + 1);
+      }
+      qk(next, c + 1);
+      weigh(cur, c);
+      asm volatile("" : "+v"(l_run));
+      float mx = tile_max(next);
+      asm volatile("" : "+v"(mx));
+      if (hidden(c + 1, j0, prefix)) {
+        hide(next, j0, prefix);
+        mx = tile_max(next);
+      }
+      move(mx);
+    };
+    int32_t c = t.t0;
+    for (; c + 2 < t.t1; c += 2) {
+      step(sa, sb, c);
+      step(sb, sa, c + 1);
+    }
+    const bool two = c + 1 < t.t1;
+    if (two) step(sa, sb, c++);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (two) weigh(sb, c);
+    else weigh(sa, c);
+
+    // A V value that is not finite in a chunk that some queries see only in part
+    // has reached the others through a weight of 0.  Where the result shows
+    // one, the tile runs again, chunk by chunk and with the same arithmetic,
+    // without such values, and each is added to the queries that see it.
+    if (!t.one) {
+      float z = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z = __builtin_fmaf(oacc[db][i], 0.f, z);
+      if (__builtin_expect(__syncthreads_or(z != 0.f), 0)) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) oacc[i] = f32x16_t{};
+        m_run = kNoMax;
+        l_run = 0.f;
+#pragma unroll 1
+        for (c = t.t0; c < t.t1; ++c) {
+          __syncthreads();
+          look_up(c);
+          issue(c);
+          wait_vmcnt<0>();
+          __syncthreads();
+          __builtin_amdgcn_sched_barrier(0);
+          qk(sa, c);
+          if (hidden(c, j0, prefix)) hide(sa, j0, prefix);
+          move(tile_max(sa));
+          u32x4_t pf[4];
+          exp_tile(sa, m_run, sc.c, l_run);
+          pack(sa, pf);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sa[kb][i] = 1.f;
+          hide(sa, j0, prefix);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sa[kb][i] = fmaxf(sa[kb][i], 0.f);
+          u32x4_t seen[4];
+          pack(sa, seen);
+          __builtin_amdgcn_sched_barrier(0);
+          const uint8_t* const vst = ring + (c & 1) * kStage + kTensor + lane * 8;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            f32x16_t above{}, below{};  // how many +inf or NaN, -inf or NaN each query sees
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              u32x4_t v = v_operand(vst, u, db), up, down;
+              split_finite<DT>(v, up, down);
+              oacc[db] = mfma32<DT>(v, pf[u], oacc[db]);
+              above = mfma32<DT>(up, seen[u], above);
+              below = mfma32<DT>(down, seen[u], below);
+              __builtin_amdgcn_sched_barrier(0);  // as few registers as it takes
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (above[i] > 0.f) oacc[db][i] += __builtin_inff();
+              if (below[i] > 0.f) oacc[db][i] -= __builtin_inff();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+  }
+
+  const float l = pair_sum(l_run);
+  if (t.parts > 1 || p.always) {
+    float* const rec = record_of<D>(a, p, w.record + w.part, kvh);
+    if (row < t.rows) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int jb = 0; jb < 4; ++jb)
+          *reinterpret_cast<f32x4_t*>(rec + row * D + db * 32 + 8 * jb + 4 * g) =
+              f32x4_t{oacc[db][4 * jb], oacc[db][4 * jb + 1], oacc[db][4 * jb + 2], oacc[db][4 * jb + 3]};
+      if (g == 0) {
+        rec[p.rows * D + row] = m_run;
+        rec[p.rows * (D + 1) + row] = l;
+      }
     }
     return;
   }
-  int32_t lo = 0, hi = R;
-  while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (a.query_starts[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  const int64_t cap = static_cast<int64_t>(a.table_width) << a.block_shift;
-  int64_t len = a.lengths[lo];
-  len = len < 0 ? 0 : (len > cap ? cap : len);
-  const int64_t pos = len - (a.query_starts[lo + 1] - t);
-  const uint16_t* const q = static_cast<const uint16_t*>(a.q) + t * a.q_token + h * a.q_head;
-  for (int i = lane; i < D; i += 64) qs[i] = widen<DT>(q[i]) * a.softmax_scale;
-  __syncthreads();
-  float m = -__builtin_inff(), l = 0.f, acc[kPer] = {};
-  // keys [k0, k1) of `blocks`
-  const auto walk = [&](const int32_t* blocks, int64_t k0, int64_t k1) {
-    for (int64_t base = k0; base < k1; base += 64) {
-      const int64_t j = base + lane < k1 ? base + lane : k1 - 1;
-      const uint32_t raw = static_cast<uint32_t>(blocks[j >> a.block_shift]);
-      const int64_t b = raw < static_cast<uint32_t>(a.num_blocks) ? raw : 0;
-      const int64_t r = j & ((1 << a.block_shift) - 1);
-      const uint16_t* k = static_cast<const uint16_t*>(a.k_cache) + b * a.ks.block + kvh * a.ks.head + r * a.ks.row;
-      const uint16_t* v = static_cast<const uint16_t*>(a.v_cache) + b * a.vs.block + kvh * a.vs.head + r * a.vs.row;
-      float s = 0.f;
-      for (int i = 0; i < D; ++i) s = __builtin_fmaf(qs[i], widen<DT>(k[i]), s);
-      const bool in = base + lane < k1;
-      float mx = in ? s : -__builtin_inff();
-      for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-      const float mn = fmaxf(m, mx);
-      const float p = in ? expf(s - mn) : 0.f;
-      const float al = m == mn ? 1.f : expf(m - mn);
-      float sum = p;
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-      l = l * al + sum;
-      m = mn;
-      for (int i = 0; i < kPer; ++i) acc[i] *= al;
-      const int64_t vp = reinterpret_cast<int64_t>(v);
-      const int n = static_cast<int>(k1 - base < 64 ? k1 - base : 64);
-      for (int jj = 0; jj < n; ++jj) {
-        const uint16_t* row = reinterpret_cast<const uint16_t*>(__shfl(vp, jj, 64));
-        const float pj = __shfl(p, jj, 64);
-        for (int i = 0; i < kPer; ++i) acc[i] = __builtin_fmaf(pj, widen<DT>(row[lane * kPer + i]), acc[i]);
-      }
+  // Output through LDS, whole rows per store.  A row that sees nothing has l = 0.
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __syncthreads();  // every wave is past its last chunk: the ring is free
+  uint8_t* const stage = ring + wave * 32 * kPitch;
+  uint8_t* const own = stage + (lane & 31) * kPitch;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int jb = 0; jb < 4; ++jb) {
+      u32x2_t o;
+      o[0] = pack2<DT>(oacc[db][4 * jb + 0] * inv, oacc[db][4 * jb + 1] * inv);
+      o[1] = pack2<DT>(oacc[db][4 * jb + 2] * inv, oacc[db][4 * jb + 3] * inv);
+      *reinterpret_cast<u32x2_t*>(own + (db * 32 + 8 * jb + 4 * g) * 2) = o;
     }
-  };
-  if (a.prefix_len > 0) walk(a.prefix_blocks, 0, a.prefix_len);
-  if (pos >= 0) {
-    const int32_t* const blocks = a.block_tables + lo * a.table_stride;
-    const int64_t last = a.causal && pos + 1 < len ? pos + 1 : len;
-    const int64_t low = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
-    walk(blocks, 0, low < a.sinks ? low : a.sinks);
-    walk(blocks, low, last);
+  __builtin_amdgcn_wave_barrier();  // a wave's LDS operations run in order
+  constexpr int kLanes = D / 8;     // lanes per row
+  constexpr int kAtOnce = 64 / kLanes;
+#pragma unroll
+  for (int k = 0; k < 32 / kAtOnce; ++k) {
+    const int r = k * kAtOnce + lane / kLanes;
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(stage + r * kPitch + (lane % kLanes) * 16);
+    if (wave * 32 + r < t.rows) {
+      const int32_t mr = t.row0 + wave * 32 + r;
+      const int32_t i = mr / group;
+      const int64_t at = (static_cast<int64_t>(t.g.first + i) * a.heads + kvh * group + (mr - i * group)) * D;
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + at + (lane % kLanes) * 8) = v;
+    }
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  for (int i = 0; i < kPer; ++i) out[lane * kPer + i] = narrow<DT>(acc[i] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[static_cast<int64_t>(h) * a.num_tokens + t] = m + logf(l);
+  if (a.lse != nullptr && g == 0 && row < t.rows)
+    a.lse[static_cast<int64_t>(kvh * group + (mat - tok * group)) * a.num_tokens + t.g.first + tok] =
+        l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------- combine
+
+// Joins the records of one row and K/V head: a wave per row, D / 64 dimensions
+// per lane.  `chunk` rows of meta per wave, of which only cut ones are joined.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs a, const PagedPass own,
+                                                            const PagedPass pre, const Scalars sc,
+                                                            const int32_t chunk) {
+  constexpr int kPer = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int32_t group = a.heads / a.kv_heads;
+  const int64_t rows = static_cast<int64_t>(live_tokens(a)) * group;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int32_t kvh = static_cast<int32_t>(id % a.kv_heads);
+  const int64_t r0 = id / a.kv_heads * chunk;
+  if (r0 >= rows) return;
+  const int n = static_cast<int>(rows - r0 < chunk ? rows - r0 : chunk);
+  int2 mo{0, 0}, mp{0, 0};
+  if (lane < n) {
+    mo = own.meta[r0 + lane];
+    if (pre.combined) mp = pre.meta[r0 + lane];
+  }
+  uint64_t todo = __ballot(lane < n && (own.always || (mo.y & 0xffff) > 1));
+  while (todo != 0) {
+    const int i = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    float m = kNoMax, l = 0.f, acc[kPer] = {};
+    auto join = [&](const PagedPass& p, int32_t record, int32_t info) {
+      const int32_t parts = info & 0xffff, row = info >> 16;
+      for (int32_t q = 0; q < parts; ++q) {
+        const float* const rec = record_of<D>(a, p, record + q, kvh);
+        const float pm = rec[p.rows * D + row], pl = rec[p.rows * (D + 1) + row];
+        const float mn = fmaxf(m, pm);
+        const float x = __builtin_amdgcn_exp2f((m - mn) * sc.c), y = __builtin_amdgcn_exp2f((pm - mn) * sc.c);
+        l = l * x + pl * y;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * x + rec[row * D + lane * kPer + k] * y;
+        m = mn;
+      }
+    };
+    if (pre.combined) join(pre, __builtin_amdgcn_readlane(mp.x, i), __builtin_amdgcn_readlane(mp.y, i));
+    join(own, __builtin_amdgcn_readlane(mo.x, i), __builtin_amdgcn_readlane(mo.y, i));
+    const int64_t mat = r0 + i;
+    const int64_t tok = mat / group;
+    const int64_t h = kvh * group + (mat - tok * group);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* const out = static_cast<uint16_t*>(a.out) + (tok * a.heads + h) * D + lane * kPer;
+    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = pack2<DT>(acc[0] * inv, acc[1] * inv);
+    else *out = static_cast<uint16_t>(pack2<DT>(acc[0] * inv, 0.f));
+    if (a.lse != nullptr && lane == 0)
+      a.lse[h * a.num_tokens + tok] =
+          l == 0.f ? -__builtin_inff() : (m * sc.c + __log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+// ---------------------------------------------------------------- launch
+
+struct Layout {
+  int32_t narrow;     // the requests' own rows by the narrow kernel
+  int32_t shared;     // a pass of its own for the prefix ...
+  int32_t shared_narrow;
+  PagedPass own, pre;
+  int64_t own_units, pre_units;  // per K/V head
+  int64_t bytes;
+};
+
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+constexpr int32_t kWideSlots = 512;
+constexpr int32_t kWideLeast = 4;
+
+Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
+                 int32_t prefix_len, void* workspace) {
+  Layout l{};
+  const int64_t group = heads / kv_heads;
+  const int64_t rows = tokens * group;
+  const int64_t busy = requests < tokens ? requests : tokens;  // requests with queries
+  l.shared = prefix_len > 0 && rows < 64 * busy;
+  l.own.rows = kWideRows;
+  l.own.least = kWideLeast;
+  l.own.wanted = (kWideSlots + kv_heads - 1) / kv_heads;
+  l.own.with_prefix = prefix_len > 0 && !l.shared;
+  l.own.always = l.shared;
+  l.own_units = rows / l.own.rows + busy + l.own.wanted;
+  const int64_t longest = (table_rows + kBN - 1) / kBN + 1 + (l.own.with_prefix ? (prefix_len + kBN - 1) / kBN : 0);
+  l.own.combined = l.shared || longest > l.own.least;
+  int64_t at = 0;
+  auto place = [&](PagedPass& p, int64_t records) {
+    char* const base = static_cast<char*>(workspace);
+    p.records = reinterpret_cast<float*>(base + at);
+    at += round256(records * kv_heads * p.rows * (dim + 2) * 4);
+    p.meta = reinterpret_cast<int2*>(base + at);
+    at += round256(rows * 8);
+  };
+  if (l.own.combined) place(l.own, 2 * l.own.wanted + 2 + (l.own.always ? rows / l.own.rows + busy : 0));
+  if (l.shared) {
+    l.pre = l.own;
+    l.pre.shared = 1;
+    l.pre.rows = kWideRows;
+    l.pre.least = kWideLeast;
+    l.pre.wanted = (kWideSlots + kv_heads - 1) / kv_heads;
+    const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
+    l.pre_units = tiles + l.pre.wanted;
+    place(l.pre, 2 * l.pre.wanted + 2 + tiles);
+  }
+  l.bytes = at;
+  return l;
+}
+
+template <int DT, int D>
+hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream) {
+  const Layout l = layout_of(a.num_tokens, a.requests, a.heads, a.kv_heads, D,
+                             static_cast<int64_t>(a.table_width) << a.block_shift, a.prefix_len, a.workspace);
+  const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
+  if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
+    return hipErrorInvalidConfiguration;
+  if (l.shared) paged_wide_kernel<DT, D><<<grid(l.pre_units), 256, 0, stream>>>(a, l.pre, sc);
+  paged_wide_kernel<DT, D><<<grid(l.own_units), 256, 0, stream>>>(a, l.own, sc);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !l.own.combined) return e;
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.heads / a.kv_heads);
+  const int32_t chunk = rows * a.kv_heads > 16384 && !l.own.always ? 64 : 1;
+  const int64_t waves = (rows + chunk - 1) / chunk * a.kv_heads;
+  if ((waves + 3) / 4 > 0x7fffffffLL / 256) return hipErrorInvalidConfiguration;
+  paged_combine_kernel<DT, D><<<dim3(static_cast<uint32_t>((waves + 3) / 4)), 256, 0, stream>>>(a, l.own, l.pre, sc,
+                                                                                             chunk);
+  return hipGetLastError();
 }
 
 }  // namespace
 
+int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                  int64_t table_rows, int32_t prefix_len) {
+  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, nullptr).bytes;
+}
+
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
   if (a.num_tokens <= 0) return hipSuccess;
-  const dim3 grid(static_cast<uint32_t>(a.num_tokens), static_cast<uint32_t>(a.heads));
-  if (a.dtype == kBF16) {
-    if (a.head_dim == 128) paged_attn_kernel<kBF16, 128><<<grid, 64, 0, stream>>>(a);
-    else paged_attn_kernel<kBF16, 64><<<grid, 64, 0, stream>>>(a);
-  } else {
-    if (a.head_dim == 128) paged_attn_kernel<kF16, 128><<<grid, 64, 0, stream>>>(a);
-    else paged_attn_kernel<kF16, 64><<<grid, 64, 0, stream>>>(a);
-  }
-  return hipGetLastError();
+  const float c = fabsf(a.softmax_scale) * kLog2e;
+  Scalars sc;
+  sc.c = c > kMinC ? c : kMinC;
+  sc.thresh = kRescaleLog2 / sc.c;
+  sc.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  if (a.dtype == kBF16)
+    return a.head_dim == 128 ? launch<kBF16, 128>(a, sc, stream) : launch<kBF16, 64>(a, sc, stream);
+  return a.head_dim == 128 ? launch<kF16, 128>(a, sc, stream) : launch<kF16, 64>(a, sc, stream);
 }
 
 }  // namespace hkv
