@@ -31,6 +31,7 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_ptr;
 typedef __attribute__((address_space(3))) void* lds_void_ptr;
 
 constexpr int kWideRows = 128;
+constexpr int kNarrowRows = 16;
 constexpr float kNoMax = -1e30f;
 
 // ---------------------------------------------------------------- plan
@@ -729,6 +730,317 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
         l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
 }
 
+// ---------------------------------------------------------------- narrow tiles
+//
+// 16 rows on the 16x16x32 MFMAs; bound by the bytes of the cache.  Two waves, each
+// with its own half (32 keys) of every chunk, its own stages in LDS and its own
+// softmax, joined at the end: no barrier in the loop.  Per stage a wave sends 32
+// rows of K and of V straight to LDS, whole rows side by side (16-byte pieces of
+// a row exchanged by its number, so that reads of one piece from 16 rows meet
+// 16 different banks).  Row addresses come from table entries that arrive in LDS the same way,
+// NS stages ahead of the rows, so no load is waited for but by count: a group is
+// the rows of stage k and the entries of stage k + NS, and NS - 1 younger groups
+// stay in flight.
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (DT == kF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                  0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                   c, 0, 0, 0);
+}
+
+// Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 of a query.
+__device__ __forceinline__ float quad_max(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return pair_max(fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
+                        __builtin_bit_cast(float, static_cast<uint32_t>(r[1]))));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return pair_sum(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])) +
+                  __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                              const Scalars sc) {
+  constexpr int kThreads = 128;
+  constexpr int kKeys = 32;                // of a stage
+  constexpr int NS = D == 128 ? 2 : 4;     // stages
+  constexpr int kRow = D * 2;              // bytes
+  constexpr int kTensor = kKeys * kRow;
+  constexpr int kStage = 2 * kTensor;
+  constexpr int NI = kTensor / 1024;       // DMAs of K, and of V, per stage
+  constexpr int kGroup = 2 * NI + 1;       // ... and one of table entries
+  constexpr int KS = D / 32;               // k-steps of S
+  constexpr int DB = D / 16;               // 16-wide blocks of O
+  constexpr int kPieces = D / 8;           // 16-byte pieces of a row
+  struct Wave {
+    uint8_t ring[NS * kStage];
+    int32_t ids[NS][64];
+    const uint8_t* rows[2][kKeys];
+  };
+  __shared__ __attribute__((aligned(1024))) Wave lds_waves[2];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int q = lane & 15;
+  const int g = lane >> 4;
+  const int32_t group = a.heads / a.kv_heads;
+  const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
+  const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
+  if (a.fill_tail && !p.shared) fill_tail<kThreads>(a);
+  const Work w = find_work<kThreads>(a, p, unit);
+  Tile t;
+  if (w.request < 0 || !make_tile(a, p, w, t)) return;
+  write_meta<kThreads>(a, p, t, w, kvh);
+
+  const int32_t mat = t.row0 + (q < t.rows ? q : t.rows - 1);
+  const int32_t tok = mat / group;
+  const int32_t head = kvh * group + (mat - tok * group);
+  const Sight mine = sight_of(a, p, t.g, tok);
+  const Sight first = sight_of(a, p, t.g, t.row0 / group);
+  const Sight last = sight_of(a, p, t.g, (t.row0 + t.rows - 1) / group);
+
+  Wave& my = lds_waves[wave];
+  const uint32_t ring_lds = lds_address(my.ring);
+  const int32_t mask = (1 << a.block_shift) - 1;
+  const int32_t n = t.t1 - t.t0;  // stages: this wave's half of each chunk
+  const auto stage_row = [&](int32_t k, bool& prefix) {
+    return chunk_row(t.keys, t.t0 + (k < n ? k : n - 1), prefix) + kKeys * wave;
+  };
+  // Lanes l and l + 32 stand for row l % 32 of a stage, one for K, one for V.
+  auto look_up = [&](int32_t k) {
+    bool prefix;
+    const int32_t j = stage_row(k, prefix) + (lane & 31);
+    dma4(t.blocks + (row_to_load(a, t.keys, j, prefix) >> a.block_shift), lds_address(my.ids[k % NS]));
+  };
+  const bool for_k = lane < 32;
+  const int64_t block_stride = for_k ? a.ks.block : a.vs.block;
+  const int64_t row_stride = for_k ? a.ks.row : a.vs.row;
+  const uint8_t* const cache = static_cast<const uint8_t*>(for_k ? a.k_cache : a.v_cache) +
+                               kvh * (for_k ? a.ks.head : a.vs.head) * 2;
+  auto issue = [&](int32_t k) {
+    bool prefix;
+    const int32_t r = row_to_load(a, t.keys, stage_row(k, prefix) + (lane & 31), prefix);
+    const int64_t b = block_of(a, my.ids[k % NS][lane]);
+    my.rows[lane >> 5][lane & 31] = cache + (b * block_stride + static_cast<int64_t>(r & mask) * row_stride) * 2;
+    const uint32_t dst = ring_lds + (k % NS) * kStage;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      constexpr int kLanes = kPieces;  // lanes of a row
+      const int row = i * (64 / kLanes) + lane / kLanes;
+      const int piece = (lane % kLanes) ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+      dma16(my.rows[0][row] + piece * 16, dst + i * 1024);
+      dma16(my.rows[1][row] + piece * 16, dst + kTensor + i * 1024);
+    }
+  };
+
+  f32x4_t oacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) oacc[i] = f32x4_t{};
+  float m_run = kNoMax, l_run = 0.f;
+  u32x4_t qf[KS];
+
+  const int k_swap = D == 128 ? q : q >> 1;
+  const int v_row = 4 * g + (q >> 2);
+  const int v_swap = D == 128 ? v_row : v_row >> 1;
+  auto scores = [&](f32x4_t (&s)[2], const uint8_t* st) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      s[kb] = f32x4_t{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kb] = mfma16<DT>(
+            *reinterpret_cast<const u32x4_t*>(st + (16 * kb + q) * kRow + (((4 * ks + g) ^ k_swap) * 16)), qf[ks], s[kb]);
+    }
+  };
+  auto hide = [&](f32x4_t (&s)[2], int32_t j0, bool prefix) {
+    const int32_t hi = (prefix ? a.prefix_len : mine.hi) - j0 - 4 * g;
+    const int32_t lo = (prefix ? 0 : mine.lo) - j0 - 4 * g;
+    const int32_t sinks = a.sinks - j0 - 4 * g;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t j = 16 * kb + i;
+        s[kb][i] = (j >= hi) | ((j < lo) & (j >= sinks)) ? -__builtin_inff() : s[kb][i];
+      }
+  };
+  auto weigh = [&](f32x4_t (&s)[2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = quad_max(mx);
+    if (__any(mx - m_run > sc.thresh)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * sc.c);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[db] *= alpha;
+      m_run = m_new;
+    }
+    const float mc = m_run * sc.c;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sc.c, -mc));
+    l_run += ((s[0][0] + s[0][1]) + (s[0][2] + s[0][3])) + ((s[1][0] + s[1][1]) + (s[1][2] + s[1][3]));
+  };
+  // P^T's k slots 8 g .. + 7 are keys 4 g .. + 3 and 16 + 4 g .. + 3, as S^T leaves the MFMA
+  auto pack = [&](const f32x4_t (&s)[2]) {
+    return u32x4_t{pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]),
+                   pack2<DT>(s[1][2], s[1][3])};
+  };
+  auto v_operand = [&](const uint8_t* st, int db) {
+    const uint8_t* const at =
+        st + kTensor + v_row * kRow + (((2 * db + ((q & 3) >> 1)) ^ v_swap) * 16) + (q & 1) * 8;
+    const u32x2_t lo = ds_read_tr(at), hi = ds_read_tr(at + 16 * kRow);
+    return u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
+
+  if (n > 0) {
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+      if (k < n) look_up(k);
+    {
+      const uint16_t* const src = static_cast<const uint16_t*>(a.q) + (t.g.first + tok) * a.q_token + head * a.q_head +
+                                  g * 8;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4_t*>(src + ks * 32);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] ^= sc.q_sign;
+    }
+    wait_vmcnt<0>();
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+      if (k < n) {
+        issue(k);
+        look_up(k + NS);
+      }
+    for (int32_t k = 0; k < n; ++k) {
+      // stage k and its successors' entries have landed; up to NS - 1 groups stay in flight
+      const int32_t rest = n - 1 - k;
+      if (rest >= NS - 1) wait_vmcnt<(NS - 1) * kGroup>();
+      else if (NS > 3 && rest == 2) wait_vmcnt<(NS > 3 ? 2 : 0) * kGroup>();
+      else if (NS > 2 && rest == 1) wait_vmcnt<(NS > 2 ? 1 : 0) * kGroup>();
+      else wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      const uint8_t* const st = my.ring + (k % NS) * kStage;
+      bool prefix;
+      const int32_t j0 = stage_row(k, prefix);
+      f32x4_t s[2];
+      scores(s, st);
+      if (!all_seen(a, first, last, j0, prefix, kKeys)) hide(s, j0, prefix);
+      weigh(s);
+      const u32x4_t pf = pack(s);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) oacc[db] = mfma16<DT>(v_operand(st, db), pf, oacc[db]);
+      if (k + NS < n) {
+        // the stage's reads are done before it is written again
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue(k + NS);
+        look_up(k + 2 * NS);
+      }
+    }
+    // Again without values that are not finite, as in the wide kernel; a wave is on its own here.
+    if (!t.one) {
+      float z = 0.f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z = __builtin_fmaf(oacc[db][i], 0.f, z);
+      if (__builtin_expect(__any(z != 0.f), 0)) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) oacc[i] = f32x4_t{};
+        m_run = kNoMax;
+        l_run = 0.f;
+#pragma unroll 1
+        for (int32_t k = 0; k < n; ++k) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          look_up(k);
+          wait_vmcnt<0>();
+          issue(k);
+          wait_vmcnt<0>();
+          asm volatile("" ::: "memory");
+          const uint8_t* const st = my.ring + (k % NS) * kStage;
+          bool prefix;
+          const int32_t j0 = stage_row(k, prefix);
+          f32x4_t s[2];
+          scores(s, st);
+          if (!all_seen(a, first, last, j0, prefix, kKeys)) hide(s, j0, prefix);
+          weigh(s);
+          const u32x4_t pf = pack(s);
+          s[0] = s[1] = f32x4_t{1.f, 1.f, 1.f, 1.f};
+          hide(s, j0, prefix);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = fmaxf(s[i >> 2][i & 3], 0.f);
+          const u32x4_t seen = pack(s);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            u32x4_t v = v_operand(st, db), up, down;
+            split_finite<DT>(v, up, down);
+            oacc[db] = mfma16<DT>(v, pf, oacc[db]);
+            const f32x4_t above = mfma16<DT>(up, seen, f32x4_t{}), below = mfma16<DT>(down, seen, f32x4_t{});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (above[i] > 0.f) oacc[db][i] += __builtin_inff();
+              if (below[i] > 0.f) oacc[db][i] -= __builtin_inff();
+            }
+          }
+        }
+      }
+    }
+  }
+  float l = quad_sum(l_run);
+
+  // wave 1's half joins wave 0's
+  float* const other = reinterpret_cast<float*>(lds_waves[1].ring);
+  if (wave == 1) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(other + (db * 64 + lane) * 4) = oacc[db];
+    other[DB * 256 + lane] = m_run;
+    other[DB * 256 + 64 + lane] = l;
+  }
+  __syncthreads();
+  if (wave == 1) return;
+  {
+    const float m1 = other[DB * 256 + lane], l1 = other[DB * 256 + 64 + lane];
+    const float m_new = fmaxf(m_run, m1);
+    const float x = __builtin_amdgcn_exp2f((m_run - m_new) * sc.c), y = __builtin_amdgcn_exp2f((m1 - m_new) * sc.c);
+    l = l * x + l1 * y;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      oacc[db] = oacc[db] * x + *reinterpret_cast<const f32x4_t*>(other + (db * 64 + lane) * 4) * y;
+    m_run = m_new;
+  }
+  if (q >= t.rows) return;
+  if (t.parts > 1 || p.always) {
+    float* const rec = record_of<D>(a, p, w.record + w.part, kvh);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(rec + q * D + db * 16 + 4 * g) = oacc[db];
+    if (g == 0) {
+      rec[p.rows * D + q] = m_run;
+      rec[p.rows * (D + 1) + q] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = (static_cast<int64_t>(t.g.first + tok) * a.heads + head) * D + 4 * g;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) store4<DT>(a.out, at + db * 16, oacc[db] * inv);
+  if (a.lse != nullptr && g == 0)
+    a.lse[static_cast<int64_t>(head) * a.num_tokens + t.g.first + tok] =
+        l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
+}
+
 // ---------------------------------------------------------------- combine
 
 // Joins the records of one row and K/V head: a wave per row, D / 64 dimensions
@@ -799,6 +1111,15 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 constexpr int32_t kWideSlots = 512;
 constexpr int32_t kWideLeast = 4;
+constexpr int32_t kNarrowSlots = 1024;
+constexpr int32_t kNarrowLeast = 4;
+
+// A launch of one kind of tile: rows, and the parts that fill the card.
+void shape(PagedPass& p, bool narrow, int32_t kv_heads) {
+  p.rows = narrow ? kNarrowRows : kWideRows;
+  p.least = narrow ? kNarrowLeast : kWideLeast;
+  p.wanted = ((narrow ? kNarrowSlots : kWideSlots) + kv_heads - 1) / kv_heads;
+}
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
                  int32_t prefix_len, void* workspace) {
@@ -807,9 +1128,8 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   const int64_t rows = tokens * group;
   const int64_t busy = requests < tokens ? requests : tokens;  // requests with queries
   l.shared = prefix_len > 0 && rows < 64 * busy;
-  l.own.rows = kWideRows;
-  l.own.least = kWideLeast;
-  l.own.wanted = (kWideSlots + kv_heads - 1) / kv_heads;
+  l.narrow = rows <= kNarrowRows * busy && !(prefix_len > 0 && !l.shared);
+  shape(l.own, l.narrow, kv_heads);
   l.own.with_prefix = prefix_len > 0 && !l.shared;
   l.own.always = l.shared;
   l.own_units = rows / l.own.rows + busy + l.own.wanted;
@@ -827,9 +1147,8 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   if (l.shared) {
     l.pre = l.own;
     l.pre.shared = 1;
-    l.pre.rows = kWideRows;
-    l.pre.least = kWideLeast;
-    l.pre.wanted = (kWideSlots + kv_heads - 1) / kv_heads;
+    l.shared_narrow = rows <= kNarrowRows;
+    shape(l.pre, l.shared_narrow, kv_heads);
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
     l.pre_units = tiles + l.pre.wanted;
     place(l.pre, 2 * l.pre.wanted + 2 + tiles);
@@ -845,12 +1164,18 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
   const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
-  if (l.shared) paged_wide_kernel<DT, D><<<grid(l.pre_units), 256, 0, stream>>>(a, l.pre, sc);
-  paged_wide_kernel<DT, D><<<grid(l.own_units), 256, 0, stream>>>(a, l.own, sc);
+  const auto run = [&](const PagedPass& p, int32_t narrow, int64_t units) {
+    if (narrow) paged_narrow_kernel<DT, D><<<grid(units), 128, 0, stream>>>(a, p, sc);
+    else paged_wide_kernel<DT, D><<<grid(units), 256, 0, stream>>>(a, p, sc);
+  };
+  if (l.shared) run(l.pre, l.shared_narrow, l.pre_units);
+  run(l.own, l.narrow, l.own_units);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !l.own.combined) return e;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.heads / a.kv_heads);
-  const int32_t chunk = rows * a.kv_heads > 16384 && !l.own.always ? 64 : 1;
+  // about 8192 waves; where every row is joined, one each
+  const int64_t per = l.own.always ? 1 : rows * a.kv_heads / 8192;
+  const int32_t chunk = static_cast<int32_t>(per < 1 ? 1 : (per > 64 ? 64 : per));
   const int64_t waves = (rows + chunk - 1) / chunk * a.kv_heads;
   if ((waves + 3) / 4 > 0x7fffffffLL / 256) return hipErrorInvalidConfiguration;
   paged_combine_kernel<DT, D><<<dim3(static_cast<uint32_t>((waves + 3) / 4)), 256, 0, stream>>>(a, l.own, l.pre, sc,
