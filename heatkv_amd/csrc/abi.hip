@@ -764,6 +764,8 @@ int32_t hkv_paged_tables(int32_t* block_tables, int64_t table_stride, const int3
       (ring_size > 0 && !free_blocks) ||
       (requests > 0 && (!lengths || !new_counts || !lengths_out || (table_width > 0 && !block_tables))))
     return fail(HKV_ERR_INVALID_ARG, "null pointer argument");
+  if ((lengths_out == lengths && requests > 0) != (range_out == free_range) && requests > 0)
+    return fail(HKV_ERR_INVALID_ARG, "lengths and free_range are updated in place both or neither");
   hkv::PagedTablesArgs a{block_tables, table_stride, lengths,     new_counts,   free_blocks, free_range, requests,
                          table_width,  ring_size,    num_tokens,  shift,        window,      sinks,      slot_map,
                          query_starts, lengths_out,  range_out,   status};

@@ -27,7 +27,7 @@ struct PagedTablesArgs {
   int32_t* query_starts;  // [requests + 1]
   int32_t* lengths_out;
   int32_t* range_out;
-  int32_t* status;
+  int32_t* status;  // [3]: status, blocks popped, blocks pushed
 };
 hipError_t launch_paged_tables(const PagedTablesArgs& a, hipStream_t stream);
 

@@ -1043,17 +1043,20 @@ __global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArg
 
 // ---------------------------------------------------------------- combine
 
-// Joins the records of one row and K/V head: a wave per row, D / 64 dimensions
-// per lane.  `chunk` rows of meta per wave, of which only cut ones are joined.
+// Joins the records of one row and K/V head: a wave per row.  Up to 64 parts at
+// once: a lane per part for the maxima and sums, then D / 4 lanes per part for its
+// values, so that all of a batch's loads are in flight together.  `chunk` rows of
+// meta per wave, of which only cut ones are joined.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs a, const PagedPass own,
                                                             const PagedPass pre, const Scalars sc,
                                                             const int32_t chunk) {
-  constexpr int kPer = D / 64;
+  constexpr int kLanes = D / 4;         // of a part's row
+  constexpr int kAtOnce = 64 / kLanes;  // parts per load
   const int lane = threadIdx.x & 63;
   const int32_t group = a.heads / a.kv_heads;
   const int64_t rows = static_cast<int64_t>(live_tokens(a)) * group;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
   const int32_t kvh = static_cast<int32_t>(id % a.kv_heads);
   const int64_t r0 = id / a.kv_heads * chunk;
   if (r0 >= rows) return;
@@ -1067,29 +1070,51 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
   while (todo != 0) {
     const int i = __builtin_ctzll(todo);
     todo &= todo - 1;
-    float m = kNoMax, l = 0.f, acc[kPer] = {};
+    float m = kNoMax, l = 0.f;
+    f32x4_t acc{};
     auto join = [&](const PagedPass& p, int32_t record, int32_t info) {
       const int32_t parts = info & 0xffff, row = info >> 16;
-      for (int32_t q = 0; q < parts; ++q) {
-        const float* const rec = record_of<D>(a, p, record + q, kvh);
-        const float pm = rec[p.rows * D + row], pl = rec[p.rows * (D + 1) + row];
-        const float mn = fmaxf(m, pm);
-        const float x = __builtin_amdgcn_exp2f((m - mn) * sc.c), y = __builtin_amdgcn_exp2f((pm - mn) * sc.c);
-        l = l * x + pl * y;
+      const int64_t stride = static_cast<int64_t>(a.kv_heads) * (p.rows * (D + 2));
+      const float* const rec0 = record_of<D>(a, p, record, kvh);
+      for (int32_t q0 = 0; q0 < parts; q0 += 64) {
+        const int32_t count = parts - q0 < 64 ? parts - q0 : 64;
+        float pm = kNoMax, pl = 0.f;
+        if (lane < count) {
+          const float* const ml = rec0 + (q0 + lane) * stride + p.rows * D + row;
+          pm = ml[0];
+          pl = ml[p.rows];
+        }
+        float mn = pm;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * x + rec[row * D + lane * kPer + k] * y;
+        for (int off = 32; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
+        mn = fmaxf(m, mn);
+        const float x = __builtin_amdgcn_exp2f((m - mn) * sc.c), y = __builtin_amdgcn_exp2f((pm - mn) * sc.c);
+        float sum = pl * y;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        l = l * x + sum;
         m = mn;
+        acc *= x;
+        const float* const o = rec0 + q0 * stride + row * D + (lane % kLanes) * 4;
+#pragma unroll 8
+        for (int32_t q = 0; q < count; q += kAtOnce) {
+          const int32_t mine = q + lane / kLanes;
+          const float z = __shfl(y, mine < count ? mine : 0, 64);
+          if (mine < count) acc += *reinterpret_cast<const f32x4_t*>(o + mine * stride) * z;
+        }
       }
     };
     if (pre.combined) join(pre, __builtin_amdgcn_readlane(mp.x, i), __builtin_amdgcn_readlane(mp.y, i));
     join(own, __builtin_amdgcn_readlane(mo.x, i), __builtin_amdgcn_readlane(mo.y, i));
+#pragma unroll
+    for (int off = kLanes; off < 64; off <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], off, 64);
     const int64_t mat = r0 + i;
     const int64_t tok = mat / group;
     const int64_t h = kvh * group + (mat - tok * group);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* const out = static_cast<uint16_t*>(a.out) + (tok * a.heads + h) * D + lane * kPer;
-    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = pack2<DT>(acc[0] * inv, acc[1] * inv);
-    else *out = static_cast<uint16_t>(pack2<DT>(acc[0] * inv, 0.f));
+    if (lane < kLanes) store4<DT>(a.out, (tok * a.heads + h) * D + lane * 4, acc * inv);
     if (a.lse != nullptr && lane == 0)
       a.lse[h * a.num_tokens + tok] =
           l == 0.f ? -__builtin_inff() : (m * sc.c + __log2f(l)) * 0.6931471805599453f;

@@ -17,25 +17,21 @@
 namespace hkv {
 namespace {
 
-constexpr int kTableThreads = 1024;
-constexpr int kTableWaves = kTableThreads / 64;
-
+// A sum of the prefix sums; saturating, so that sums past 32 bits refuse the step.
 struct Sum3 {
-  int64_t tokens, popped, pushed;
+  uint32_t tokens, popped, pushed;
 };
 
 __device__ __forceinline__ Sum3 add(const Sum3& a, const Sum3& b) {
-  return Sum3{a.tokens + b.tokens, a.popped + b.popped, a.pushed + b.pushed};
+  return Sum3{__builtin_elementwise_add_sat(a.tokens, b.tokens), __builtin_elementwise_add_sat(a.popped, b.popped),
+              __builtin_elementwise_add_sat(a.pushed, b.pushed)};
 }
 
 // What one request does in a step.
 struct Request {
-  int64_t held;  // rows before the step
-  int64_t n;     // new tokens
-  int64_t have, need;
+  int64_t have, need;  // blocks
   int64_t front;       // ended: blocks [0, front) are pushed, too
   int64_t from, to;    // logical blocks [from, to) are pushed
-  bool ended;
 };
 
 // First block that the tokens from position `rows` on still see behind the sinks.
@@ -45,34 +41,32 @@ __device__ __forceinline__ int64_t first_live(int64_t rows, int64_t kept, const 
   return b > kept ? b : kept;
 }
 
-__device__ __forceinline__ Request load_request(const PagedTablesArgs& a, int32_t r) {
+// A request that holds `held` rows and brings n tokens, or (n < 0) has ended.
+__device__ __forceinline__ Request request_of(const PagedTablesArgs& a, int64_t held, int64_t n) {
   Request q;
-  const int32_t count = a.new_counts[r];
-  const int32_t len = a.lengths[r];
   const int64_t block = 1LL << a.block_shift;
-  q.ended = count < 0;
-  q.n = count > 0 ? count : 0;
-  q.held = len > 0 ? len : 0;
-  q.have = (q.held + block - 1) >> a.block_shift;
-  q.need = (q.held + q.n + block - 1) >> a.block_shift;
+  const bool ended = n < 0;
+  if (ended) n = 0;
+  q.have = (held + block - 1) >> a.block_shift;
+  q.need = (held + n + block - 1) >> a.block_shift;
   const int64_t kept = a.window > 0 ? (a.sinks + block - 1) >> a.block_shift : 0;
   q.front = 0;
   q.from = 0;
   q.to = 0;
-  if (q.ended) {
-    const int64_t low = a.window > 0 ? first_live(q.held, kept, a) : 0;
+  if (ended) {
+    const int64_t low = a.window > 0 ? first_live(held, kept, a) : 0;
     q.front = kept < q.have ? kept : q.have;
     q.from = low < q.have ? low : q.have;
     q.to = q.have;
   } else if (a.window > 0) {
-    q.from = first_live(q.held, kept, a);
-    q.to = first_live(q.held + q.n, kept, a);
+    q.from = first_live(held, kept, a);
+    q.to = first_live(held + n, kept, a);
   }
   return q;
 }
 
 // The r with prefix[r] <= i < prefix[r + 1]; prefix[0] = 0 <= i < prefix[n].
-__device__ __forceinline__ int32_t find(const int32_t* prefix, int32_t n, int32_t i) {
+__device__ __forceinline__ int32_t find(const uint32_t* prefix, int32_t n, uint32_t i) {
   int32_t lo = 0, hi = n;
   while (hi - lo > 1) {
     const int32_t mid = (lo + hi) >> 1;
@@ -91,102 +85,146 @@ __device__ __forceinline__ Sum3 wave_scan(Sum3 v) {
   return v;
 }
 
-__global__ __launch_bounds__(kTableThreads) void paged_tables_kernel(PagedTablesArgs a) {
-  __shared__ int32_t starts[kMaxRequests + 1], popped[kMaxRequests + 1], pushed[kMaxRequests + 1];
-  __shared__ Sum3 wave_total[kTableWaves];
+// Every workgroup computes the prefix sums of all requests for itself (a few
+// thousand integers) and takes its share of the blocks and tokens, so that one
+// launch does it all: no workgroup reads what another writes.  Popped are table
+// entries behind those held, pushed ring entries behind those free; only where
+// free and pushed together exceed the ring (a prompt longer than its window on an
+// almost empty cache) would a push meet an entry yet to be popped, and there the first
+// workgroup takes everything, in order.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void paged_tables_kernel(const PagedTablesArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr int32_t kEnded = static_cast<int32_t>(0x80000000u);
+  __shared__ uint32_t starts[kMaxRequests + 1], popped[kMaxRequests + 1], pushed[kMaxRequests + 1];
+  __shared__ int32_t rows[kMaxRequests];  // held, kEnded set where the request has ended
+  __shared__ Sum3 wave_total[kWaves];
   __shared__ int32_t too_long;
   const int tid = threadIdx.x;
   const int wave = tid >> 6;
   const int32_t R = a.requests, N = a.ring_size;
-  int32_t first = a.free_range[0], free = a.free_range[1];
-  free = free < 0 ? 0 : (free > N ? N : free);
-  first = N > 0 ? first % N : 0;
-  if (first < 0) first += N;
+  const int32_t given0 = a.free_range[0], given1 = a.free_range[1];
   if (tid == 0) too_long = 0;
-  __syncthreads();
   Sum3 carry{0, 0, 0};
-  for (int32_t r0 = 0; r0 < R; r0 += kTableThreads) {
+  for (int32_t r0 = 0; r0 < R || r0 == 0; r0 += kThreads) {
     const int32_t r = r0 + tid;
     Sum3 mine{0, 0, 0};
+    bool over = false;
     if (r < R) {
-      const Request q = load_request(a, r);
-      mine = Sum3{q.n, q.need - q.have, q.front + q.to - q.from};
-      if (q.need > a.table_width || q.have > a.table_width || q.held + q.n > 0x7fffffffLL) too_long = 1;
+      const int32_t n = a.new_counts[r];
+      int32_t held = a.lengths[r];
+      held = held > 0 ? held : 0;
+      const Request q = request_of(a, held, n);
+      const int64_t push = q.front + q.to - q.from;
+      mine = Sum3{n > 0 ? static_cast<uint32_t>(n) : 0u, static_cast<uint32_t>(q.need - q.have),
+                  static_cast<uint32_t>(push)};
+      over = q.need > a.table_width || held + (n > 0 ? static_cast<int64_t>(n) : 0) > 0x7fffffffLL;
+      rows[r] = n < 0 ? held | kEnded : held;
     }
     const Sum3 incl = wave_scan(mine);
     if ((tid & 63) == 63) wave_total[wave] = incl;
-    __syncthreads();
-    Sum3 before = carry;
-    for (int w = 0; w < kTableWaves; ++w) {
-      if (w == wave) before = add(before, incl);
-      carry = add(carry, wave_total[w]);
+    __syncthreads();  // also the first: too_long is clear
+    if (over) too_long = 1;
+    Sum3 before = add(carry, incl);
+    for (int w = 0; w < kWaves; ++w) {
       if (w < wave) before = add(before, wave_total[w]);
+      carry = add(carry, wave_total[w]);
     }
     if (r < R) {
-      // sums past 32 bits refuse the step below
-      starts[r + 1] = static_cast<int32_t>(before.tokens);
-      popped[r + 1] = static_cast<int32_t>(before.popped);
-      pushed[r + 1] = static_cast<int32_t>(before.pushed);
+      starts[r + 1] = before.tokens;
+      popped[r + 1] = before.popped;
+      pushed[r + 1] = before.pushed;
     }
+    if (r == 0) starts[0] = popped[0] = pushed[0] = 0;
     __syncthreads();
   }
-  if (tid == 0) starts[0] = popped[0] = pushed[0] = 0;
-  __syncthreads();
-  const int32_t status =
-      (carry.popped > free ? 1 : 0) | (too_long != 0 ? 2 : 0) | (carry.tokens > a.num_tokens ? 4 : 0);
-  const bool fine = status == 0;
-  // lengths_out may be lengths, so each is read before it is written and not again
-  const auto ring_at = [&](int64_t i) { return static_cast<int32_t>((first + i) % N); };
-  if (fine) {
-    for (int32_t i = tid; i < static_cast<int32_t>(carry.popped); i += kTableThreads) {
-      const int32_t r = find(popped, R, i);
-      const Request q = load_request(a, r);
-      a.block_tables[r * a.table_stride + q.have + (i - popped[r])] = a.free_blocks[ring_at(i)];
+  int32_t free = given1 < 0 ? 0 : (given1 > N ? N : given1);
+  int32_t first = N > 0 ? given0 % N : 0;
+  if (first < 0) first += N;
+  const int64_t left = static_cast<int64_t>(free) - carry.popped + carry.pushed;
+  const int32_t status = (carry.popped > static_cast<uint32_t>(free) ? 1 : 0) | (too_long != 0 ? 2 : 0) |
+                         (carry.tokens > static_cast<uint32_t>(a.num_tokens) ? 4 : 0);
+  // blocks given back that the ring has no room for: not the blocks of this cache
+  const int32_t state = status == 0 && left > N ? 8 : status;
+  const bool fine = state == 0;
+  const auto ring_at = [&](int64_t i) {
+    int64_t at = first + i;  // i < 2 N
+    if (at >= N) at -= N;
+    if (at >= N) at -= N;
+    return at;
+  };
+  const bool alone = static_cast<int64_t>(free) + carry.pushed > N;
+  const int64_t step = alone ? kThreads : static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t at = alone ? tid : static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+  if (blockIdx.x == 0) {
+    for (int32_t r = tid; r <= R; r += kThreads) a.query_starts[r] = fine ? static_cast<int32_t>(starts[r]) : 0;
+    if (a.lengths_out != a.lengths) {
+      for (int32_t r = tid; r < R; r += kThreads) {
+        const int32_t n = static_cast<int32_t>(starts[r + 1] - starts[r]);
+        a.lengths_out[r] = !fine ? a.lengths[r] : (rows[r] & kEnded) != 0 ? 0 : rows[r] + n;
+      }
     }
-    for (int32_t i = tid; i < static_cast<int32_t>(carry.pushed); i += kTableThreads) {
-      const int32_t r = find(pushed, R, i);
-      const Request q = load_request(a, r);
-      const int32_t k = i - pushed[r];
-      const int64_t j = k < q.front ? k : q.from + (k - q.front);
-      // a block that this step pops is read where it is popped from
-      const int32_t b = j < q.have ? a.block_tables[r * a.table_stride + j]
-                                   : a.free_blocks[ring_at(popped[r] + (j - q.have))];
-      a.free_blocks[ring_at(static_cast<int64_t>(free) + i)] = b;
+    if (tid == 0) {
+      a.status[0] = state;
+      a.status[1] = fine ? static_cast<int32_t>(carry.popped) : 0;
+      a.status[2] = fine ? static_cast<int32_t>(carry.pushed) : 0;
+      if (a.range_out != a.free_range) {
+        a.range_out[0] = fine && N > 0 ? static_cast<int32_t>(ring_at(carry.popped)) : given0;
+        a.range_out[1] = fine ? static_cast<int32_t>(left) : given1;
+      }
     }
   }
-  __syncthreads();
-  for (int32_t r = tid; r < R; r += kTableThreads) {
-    const Request q = load_request(a, r);
-    const int32_t after = q.ended ? 0 : static_cast<int32_t>(q.held + q.n);
-    const int32_t was = a.lengths[r];
-    a.query_starts[r] = fine ? starts[r] : 0;
-    a.lengths_out[r] = fine ? after : was;
+  if (alone && blockIdx.x != 0) return;
+  const auto request = [&](int32_t r) {
+    const int32_t x = rows[r];
+    return (x & kEnded) != 0 ? request_of(a, x & ~kEnded, -1) : request_of(a, x, starts[r + 1] - starts[r]);
+  };
+  // Slot of each token: its request's block of the row, and the row in it.
+  for (int64_t t = at; t < a.num_tokens; t += step) {
+    int64_t slot = -1;
+    if (fine && t < carry.tokens) {
+      const int32_t r = find(starts, R, static_cast<uint32_t>(t));
+      const int64_t row = (rows[r] & ~kEnded) + (t - starts[r]);
+      const int64_t j = row >> a.block_shift;
+      const int64_t have = ((rows[r] & ~kEnded) + (1LL << a.block_shift) - 1) >> a.block_shift;
+      const int64_t b = j < have ? a.block_tables[r * a.table_stride + j]
+                                 : a.free_blocks[ring_at(popped[r] + (j - have))];
+      slot = (b << a.block_shift) + (row & ((1LL << a.block_shift) - 1));
+    }
+    a.slot_map[t] = slot;
   }
-  if (tid == 0) {
-    a.query_starts[R] = fine ? starts[R] : 0;
-    a.status[0] = status;
-    const int32_t f0 = a.free_range[0], f1 = a.free_range[1];
-    a.range_out[0] = fine ? (N > 0 ? ring_at(carry.popped) : 0) : f0;
-    a.range_out[1] = fine ? static_cast<int32_t>(free - carry.popped + carry.pushed) : f1;
+  if (!fine) return;
+  for (int64_t i = at; i < carry.popped; i += step) {
+    const int32_t r = find(popped, R, static_cast<uint32_t>(i));
+    a.block_tables[r * a.table_stride + request(r).have + (i - popped[r])] = a.free_blocks[ring_at(i)];
+  }
+  if (alone) __syncthreads();
+  for (int64_t i = at; i < carry.pushed; i += step) {
+    const int32_t r = find(pushed, R, static_cast<uint32_t>(i));
+    const Request q = request(r);
+    const int64_t k = i - pushed[r];
+    const int64_t j = k < q.front ? k : q.from + (k - q.front);
+    // a block that this step pops is read where it is popped from, or (alone) to
+    const int32_t b = j < q.have || alone ? a.block_tables[r * a.table_stride + j]
+                                          : a.free_blocks[ring_at(popped[r] + (j - q.have))];
+    a.free_blocks[ring_at(static_cast<int64_t>(free) + i)] = b;
   }
 }
 
-// Slot of each token: its request's block of the row, and the row in it.
-__global__ __launch_bounds__(256) void paged_slots_kernel(PagedTablesArgs a) {
-  __shared__ int32_t starts[kMaxRequests + 1];
-  const int32_t R = a.requests;
-  for (int32_t r = threadIdx.x; r <= R; r += 256) starts[r] = a.query_starts[r];
-  __syncthreads();
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < a.num_tokens;
-       t += static_cast<int64_t>(gridDim.x) * 256) {
-    int64_t slot = -1;
-    if (t < starts[R]) {
-      const int32_t r = find(starts, R, static_cast<int32_t>(t));
-      const int32_t row = a.lengths_out[r] - starts[r + 1] + static_cast<int32_t>(t);
-      const int64_t b = a.block_tables[r * a.table_stride + (row >> a.block_shift)];
-      slot = (b << a.block_shift) + (row & ((1 << a.block_shift) - 1));
-    }
-    a.slot_map[t] = slot;
+// The state in place, once no workgroup of the step reads the old one any more.
+__global__ __launch_bounds__(256) void paged_state_kernel(const PagedTablesArgs a) {
+  if (a.status[0] != 0) return;
+  for (int32_t r = threadIdx.x; r < a.requests; r += 256) {
+    const int32_t held = a.lengths[r] > 0 ? a.lengths[r] : 0;
+    a.lengths_out[r] = a.new_counts[r] < 0 ? 0 : held + (a.query_starts[r + 1] - a.query_starts[r]);
+  }
+  if (threadIdx.x == 0 && a.ring_size > 0) {
+    const int64_t N = a.ring_size;
+    const int32_t given0 = a.free_range[0], given1 = a.free_range[1];
+    int64_t first = given0 % N;
+    if (first < 0) first += N;
+    a.range_out[0] = static_cast<int32_t>((first + a.status[1]) % N);
+    a.range_out[1] = (given1 < 0 ? 0 : given1) - a.status[1] + a.status[2];
   }
 }
 
@@ -220,11 +258,16 @@ typedef uint32_t U16B __attribute__((ext_vector_type(4)));
 }  // namespace
 
 hipError_t launch_paged_tables(const PagedTablesArgs& a, hipStream_t stream) {
-  paged_tables_kernel<<<1, kTableThreads, 0, stream>>>(a);
+  // a workgroup per 1024 tokens, or per 32 requests whose blocks may move
+  int64_t blocks = (a.num_tokens + 1023LL) / 1024;
+  if (blocks < a.requests / 32) blocks = a.requests / 32;
+  blocks = blocks < 1 ? 1 : (blocks > 128 ? 128 : blocks);
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  if (a.requests <= 256 && blocks == 1) paged_tables_kernel<256><<<grid, 256, 0, stream>>>(a);
+  else paged_tables_kernel<1024><<<grid, 1024, 0, stream>>>(a);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.num_tokens == 0) return e;
-  const int64_t blocks = (a.num_tokens + 255LL) / 256;
-  paged_slots_kernel<<<dim3(static_cast<uint32_t>(blocks < 1024 ? blocks : 1024)), 256, 0, stream>>>(a);
+  if (e != hipSuccess || (a.lengths_out != a.lengths && a.range_out != a.free_range)) return e;
+  paged_state_kernel<<<1, 256, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -147,8 +147,8 @@ def build_paged_tables(
     int32 ``[R + 1]``, the new ``lengths`` and ``free_range`` (new tensors, or
     with ``in_place`` the given ones, updated) and ``status`` int32 ``[1]``: 0,
     or a sum of 1 (too few free blocks), 2 (a request does not fit its table
-    row) and 4 (more tokens than ``num_tokens``).  A step with a nonzero status
-    changes nothing: every slot is -1, every query start 0, and the state is
+    row) and 4 (more tokens than ``num_tokens``), or 8 (more blocks given back
+    than the ring has room for).  A step with a nonzero status changes nothing: every slot is -1, every query start 0, and the state is
     as before.  Calling it again with the same inputs gives the same results
     (unless ``in_place``).
     """
@@ -171,14 +171,14 @@ def build_paged_tables(
     _lib.require_device(device)
     slot_map = torch.empty((num_tokens,), dtype=torch.int64, device=device)
     query_starts = torch.empty((R + 1,), dtype=torch.int32, device=device)
-    status = torch.empty((1,), dtype=torch.int32, device=device)
+    status = torch.empty((3,), dtype=torch.int32, device=device)
     lengths_out = lengths if in_place else torch.empty_like(lengths)
     range_out = free_range if in_place else torch.empty_like(free_range)
     _call(device, _lib.load().hkv_paged_tables, block_tables.data_ptr(), int(block_tables.stride(0)),
           lengths.data_ptr(), new_counts.data_ptr(), free_blocks.data_ptr(), free_range.data_ptr(), R, M,
           int(free_blocks.shape[0]), num_tokens, block_size, window, sinks, slot_map.data_ptr(),
           query_starts.data_ptr(), lengths_out.data_ptr(), range_out.data_ptr(), status.data_ptr())
-    return PagedStep(slot_map, query_starts, lengths_out, range_out, status)
+    return PagedStep(slot_map, query_starts, lengths_out, range_out, status[:1])
 
 
 def append_paged_kv(

@@ -454,11 +454,13 @@ int32_t hkv_qkv_produce(const void* qkv, int64_t token_stride, const float* q_bi
  *   slot_map [num_tokens] : block * block_size + row of each token, in request
  *       order; -1 behind the last
  *   query_starts [requests + 1] : first token of each request
- *   lengths_out, range_out : the state after the step (may be lengths, free_range)
- *   status [1] : 0, or a sum of 1 (too few free blocks), 2 (a request does not
- *       fit its table row), 4 (more tokens than num_tokens); then nothing is
- *       popped, pushed or entered, the state is as before, every slot is -1 and every
- *       query start 0.
+ *   lengths_out, range_out : the state after the step (may both be lengths and
+ *       free_range themselves)
+ *   status [3] : 0, blocks popped, blocks pushed; or a sum of 1 (too few free
+ *       blocks), 2 (a request does not fit its table row), 4 (more tokens than
+ *       num_tokens), or 8 (more blocks given back than the ring has room for);
+ *       then nothing is popped, pushed or entered, the state is as before, every slot
+ *       is -1 and every query start 0.
  */
 int32_t hkv_paged_tables(int32_t* block_tables, int64_t table_stride, const int32_t* lengths,
                          const int32_t* new_counts, int32_t* free_blocks, const int32_t* free_range,

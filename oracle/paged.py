@@ -26,6 +26,7 @@ def build_tables(tables, lengths, new_counts, ring, ring_range, num_tokens, bloc
     if sum(fresh) > num_tokens:
         status |= 4
     slots = np.full(num_tokens, -1, np.int64)
+    given = np.array(tables), np.array(ring)
     if status:
         return (tables, ring, slots, np.zeros(R + 1, np.int32), np.array(lengths, np.int32),
                 np.array(ring_range, np.int32), status)
@@ -51,6 +52,9 @@ def build_tables(tables, lengths, new_counts, ring, ring_range, num_tokens, bloc
             pushed += [tables[r, j] for j in range(blocks_of(held)) if needed(j, held)]
         else:
             pushed += [tables[r, j] for j in range(blocks_of(held + n)) if needed(j, held) and not needed(j, held + n)]
+    if free - popped + len(pushed) > N:  # more than the ring has room for
+        return (*given, np.full(num_tokens, -1, np.int64), np.zeros(R + 1, np.int32), np.array(lengths, np.int32),
+                np.array(ring_range, np.int32), 8)
     for i, b in enumerate(pushed):
         ring[(first + free + i) % N] = b
     new_range = np.array([(first + popped) % N if N else 0, free - popped + len(pushed)], np.int32)

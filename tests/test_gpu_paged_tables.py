@@ -96,6 +96,26 @@ def test_refused_steps_change_nothing(device, counts, tokens, status):
     assert s.step([1, 1, -1], 12) == 0
 
 
+@pytest.mark.parametrize("requests", [2, 600])
+def test_prompt_longer_than_its_window_on_a_full_ring(device, requests):
+    """Blocks popped and pushed in one step, on a ring without room for both."""
+    s = State(requests, 64, 20 + requests, 4)
+    counts = np.zeros(requests, int)
+    counts[0] = 70
+    assert s.step(counts, 70, window=8, sinks=3) == 0
+    counts[:] = 1
+    assert s.step(counts, requests, window=8, sinks=3, in_place=True) == 0
+    counts[0], counts[1] = -1, 75
+    assert s.step(counts, 2 * requests + 75, window=8, sinks=3) == 0
+
+
+def test_blocks_that_the_ring_has_no_room_for(device):
+    s = State(2, 8, 4, 4)
+    s.tables[0, :6], s.lengths[0] = np.arange(6), 22
+    assert s.step([-1, 3], 5) == 8
+    assert s.step([-1, 3], 5, in_place=True) == 8
+
+
 def test_no_requests_no_tokens(device):
     s = State(2, 4, 8, 4)
     assert s.step([0, 0], 0) == 0
