@@ -799,16 +799,17 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
 
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
-                                            int32_t prefix_length) {
+                                            int32_t prefix_length, int32_t window, int32_t sinks) {
   const int32_t shift = block_shift_of(block_size);
   if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
   if (num_tokens < 0 || requests < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || table_width < 0 ||
-      prefix_length < 0)
-    return fail(HKV_ERR_INVALID_ARG, "negative size, or heads no multiple of kv_heads");
+      prefix_length < 0 || window < 0 || sinks < 0)
+    return fail(HKV_ERR_INVALID_ARG, "negative size, window or sinks, or heads no multiple of kv_heads");
   ok();
   return num_tokens == 0 ? 0
                          : hkv::paged_attention_workspace(num_tokens, requests, heads, kv_heads, head_dim,
-                                                          static_cast<int64_t>(table_width) << shift, prefix_length);
+                                                          static_cast<int64_t>(table_width) << shift, prefix_length, window,
+                                                          sinks);
 }
 
 int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -854,7 +855,7 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
   if (strides % 8 != 0 || ptrs % 16 != 0)
     return fail(HKV_ERR_INVALID_ARG, "q, the caches and out must start at, and their rows lie, 16 bytes apart");
   const int64_t need = hkv_paged_attention_workspace_bytes(num_tokens, requests, heads, kv_heads, head_dim,
-                                                           table_width, block_size, prefix_length);
+                                                           table_width, block_size, prefix_length, window, sinks);
   if (need < 0) return static_cast<int32_t>(need);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256))
     return fail(HKV_ERR_INVALID_ARG, "the call needs %lld bytes of 256-byte aligned workspace",

@@ -87,6 +87,6 @@ struct PagedAttnArgs {
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                                  int64_t table_rows, int32_t prefix_len);
+                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks);
 
 }  // namespace hkv

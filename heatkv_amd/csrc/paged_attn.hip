@@ -43,7 +43,9 @@ struct PagedPass {
   int32_t with_prefix;  // each tile's keys begin with the prefix (wide tiles that need no sharing)
   int32_t rows;      // rows of a tile
   int32_t least;     // chunks of a part at least
-  int32_t wanted;    // units per K/V head that fill the card
+  int32_t wanted;    // units per K/V head that fill the card once
+  int32_t most;      // ... and that parts may make at most
+  int32_t cap;       // chunks of a part from which more than `wanted` are made
   int32_t always;    // every tile leaves records (a shared prefix is joined to it)
   int32_t combined;  // a combine launch follows: write meta
   float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
@@ -51,6 +53,17 @@ struct PagedPass {
 };
 
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Chunks of a part in a launch of `total` chunks (per K/V head): total / c, the
+// number of parts, never falls with total and is at most `most`.
+__host__ __device__ __forceinline__ int64_t part_chunks(const PagedPass& p, int64_t total) {
+  int64_t c = (total + p.wanted - 1) / p.wanted;
+  if (c > p.cap) {
+    c = (total + p.most - 1) / p.most;
+    c = c > p.cap ? c : p.cap;
+  }
+  return c > p.least ? c : p.least;
+}
 
 struct Geometry {
   int32_t n;      // queries
@@ -131,6 +144,7 @@ struct Work {
   int32_t part;
   int32_t parts;    // of the request's tiles
   int32_t record;   // of the tile's part 0
+  Geometry g;       // of the request
 };
 
 __device__ __forceinline__ int32_t parts_of(const Load& l, int64_t c) {
@@ -166,13 +180,16 @@ template <int kThreads>
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
-  Work w{-1, 0, 0, 1, 0};
+  Work w{-1, 0, 0, 1, 0, {0, 0, 0}};
   if (R <= 64) {
     Load l{0, 0};
-    if (lane < R) l = load_of(a, p, load_request(a, p, lane));
+    Geometry g{0, 0, 0};
+    if (lane < R) {
+      g = load_request(a, p, lane);
+      l = load_of(a, p, g);
+    }
     const int64_t total = wave_sum64(static_cast<int64_t>(l.tiles) * l.chunks);
-    int64_t c = (total + p.wanted - 1) / p.wanted;
-    c = c < p.least ? p.least : c;
+    const int64_t c = part_chunks(p, total);
     const int2 mine = units_of(p, l, c);
     const int2 end = wave_prefix(mine);
     const uint64_t hit = __ballot(unit >= end.x - mine.x && unit < end.x);
@@ -185,12 +202,14 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
     w.part = in % parts;
     w.tile = __builtin_amdgcn_readlane(l.tiles, src) - 1 - in / parts;  // causal tiles: longest first
     w.record = __builtin_amdgcn_readlane(end.y - mine.y, src) + w.tile * parts;
+    w.g = Geometry{__builtin_amdgcn_readlane(g.n, src), __builtin_amdgcn_readlane(g.first, src),
+                   __builtin_amdgcn_readlane(g.len, src)};
     return w;
   }
   constexpr int kWaves = kThreads / 64;
   __shared__ int64_t wave_total[kWaves];
   __shared__ int2 wave_units[kWaves];
-  __shared__ int32_t found[5];
+  __shared__ int32_t found[8];
   const int tid = threadIdx.x;
   const int wave = tid >> 6;
   const int32_t run = (R + kThreads - 1) / kThreads;
@@ -206,8 +225,7 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
   __syncthreads();
   int64_t total = 0;
   for (int i = 0; i < kWaves; ++i) total += wave_total[i];
-  int64_t c = (total + p.wanted - 1) / p.wanted;
-  c = c < p.least ? p.least : c;
+  const int64_t c = part_chunks(p, total);
   int2 mine{0, 0};
   for (int32_t r = r0; r < r1; ++r) {
     const int2 u = units_of(p, load_of(a, p, load_request(a, p, r)), c);
@@ -220,7 +238,8 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
   int2 at{end.x - mine.x, end.y - mine.y};
   if (unit >= at.x && unit < end.x) {  // one thread
     for (int32_t r = r0; r < r1; ++r) {
-      const Load l = load_of(a, p, load_request(a, p, r));
+      const Geometry g = load_request(a, p, r);
+      const Load l = load_of(a, p, g);
       const int2 u = units_of(p, l, c);
       if (unit < at.x + u.x) {
         const int32_t parts = parts_of(l, c);
@@ -230,6 +249,9 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
         found[2] = in % parts;
         found[3] = parts;
         found[4] = at.y + found[1] * parts;
+        found[5] = g.n;
+        found[6] = g.first;
+        found[7] = g.len;
         break;
       }
       at = int2{at.x + u.x, at.y + u.y};
@@ -242,6 +264,7 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
   w.part = __builtin_amdgcn_readfirstlane(found[2]);
   w.parts = __builtin_amdgcn_readfirstlane(found[3]);
   w.record = __builtin_amdgcn_readfirstlane(found[4]);
+  w.g = Geometry{uniform(found[5]), uniform(found[6]), uniform(found[7])};
   return w;
 }
 
@@ -260,10 +283,7 @@ struct Tile {
 // Whether there is work; part and tile of `w` as its tile cuts them.
 __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPass& p, const Work& w, Tile& t) {
   const int32_t group = a.heads / a.kv_heads;
-  t.g = load_request(a, p, w.request);
-  t.g.n = uniform(t.g.n);
-  t.g.first = uniform(t.g.first);
-  t.g.len = uniform(t.g.len);
+  t.g = w.g;
   t.row0 = w.tile * p.rows;
   t.rows = t.g.n * group - t.row0;
   t.rows = t.rows < p.rows ? t.rows : p.rows;
@@ -765,12 +785,11 @@ __device__ __forceinline__ float quad_sum(float v) {
                   __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
+template <int DT, int D, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
                                                               const Scalars sc) {
-  constexpr int kThreads = 128;
+  constexpr int kThreads = NW * 64;
   constexpr int kKeys = 32;                // of a stage
-  constexpr int NS = D == 128 ? 2 : 4;     // stages
   constexpr int kRow = D * 2;              // bytes
   constexpr int kTensor = kKeys * kRow;
   constexpr int kStage = 2 * kTensor;
@@ -784,7 +803,7 @@ __global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArg
     int32_t ids[NS][64];
     const uint8_t* rows[2][kKeys];
   };
-  __shared__ __attribute__((aligned(1024))) Wave lds_waves[2];
+  __shared__ __attribute__((aligned(1024))) Wave lds_waves[NW];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -810,15 +829,17 @@ __global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArg
   Wave& my = lds_waves[wave];
   const uint32_t ring_lds = lds_address(my.ring);
   const int32_t mask = (1 << a.block_shift) - 1;
-  const int32_t n = t.t1 - t.t0;  // stages: this wave's half of each chunk
+  // the part's 32-key halves of chunks are dealt to the waves in turn
+  const int32_t n = (2 * (t.t1 - t.t0) - wave + NW - 1) / NW;
   const auto stage_row = [&](int32_t k, bool& prefix) {
-    return chunk_row(t.keys, t.t0 + (k < n ? k : n - 1), prefix) + kKeys * wave;
+    const int32_t s = (k < n ? k : n - 1) * NW + wave;
+    return chunk_row(t.keys, t.t0 + (s >> 1), prefix) + kKeys * (s & 1);
   };
   // Lanes l and l + 32 stand for row l % 32 of a stage, one for K, one for V.
   auto look_up = [&](int32_t k) {
     bool prefix;
     const int32_t j = stage_row(k, prefix) + (lane & 31);
-    dma4(t.blocks + (row_to_load(a, t.keys, j, prefix) >> a.block_shift), lds_address(my.ids[k % NS]));
+    dma4((prefix ? a.prefix_blocks : t.blocks) + (row_to_load(a, t.keys, j, prefix) >> a.block_shift), lds_address(my.ids[k % NS]));
   };
   const bool for_k = lane < 32;
   const int64_t block_stride = for_k ? a.ks.block : a.vs.block;
@@ -1001,17 +1022,19 @@ __global__ __launch_bounds__(128, 1) void paged_narrow_kernel(const PagedAttnArg
   }
   float l = quad_sum(l_run);
 
-  // wave 1's half joins wave 0's
-  float* const other = reinterpret_cast<float*>(lds_waves[1].ring);
-  if (wave == 1) {
+  // the other waves' results join wave 0's, in their order
+  float* const left = reinterpret_cast<float*>(my.ring);
+  if (wave != 0) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(other + (db * 64 + lane) * 4) = oacc[db];
-    other[DB * 256 + lane] = m_run;
-    other[DB * 256 + 64 + lane] = l;
+    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(left + (db * 64 + lane) * 4) = oacc[db];
+    left[DB * 256 + lane] = m_run;
+    left[DB * 256 + 64 + lane] = l;
   }
   __syncthreads();
-  if (wave == 1) return;
-  {
+  if (wave != 0) return;
+#pragma unroll
+  for (int v = 1; v < NW; ++v) {
+    const float* const other = reinterpret_cast<const float*>(lds_waves[v].ring);
     const float m1 = other[DB * 256 + lane], l1 = other[DB * 256 + 64 + lane];
     const float m_new = fmaxf(m_run, m1);
     const float x = __builtin_amdgcn_exp2f((m_run - m_new) * sc.c), y = __builtin_amdgcn_exp2f((m1 - m_new) * sc.c);
@@ -1123,10 +1146,31 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
 
 // ---------------------------------------------------------------- launch
 
+#ifndef XWL
+#define XWL 8
+#endif
+#ifndef XLONG
+#define XLONG 16
+#endif
+#ifndef XSHORT
+#define XSHORT 16
+#endif
+#ifndef XCONCAT
+#define XCONCAT 2048
+#endif
+// What runs a launch's tiles.
+enum Form : int32_t {
+  kWide,         // paged_wide_kernel, two workgroups per CU
+  kNarrowMany,   // paged_narrow_kernel, 2 waves, two workgroups per CU
+  kNarrowLong,   // ... 4 waves, one per CU
+  kNarrowAlone,  // ... 8 waves with one stage each, one per CU; no tile is cut
+};
+constexpr int32_t kUncut = XSHORT;      // chunks of a tile that kNarrowAlone takes
+constexpr int32_t kLongUnit = XLONG;   // chunks of a unit from which kNarrowLong is taken
+
 struct Layout {
-  int32_t narrow;     // the requests' own rows by the narrow kernel
-  int32_t shared;     // a pass of its own for the prefix ...
-  int32_t shared_narrow;
+  int32_t shared;  // a pass of its own for the prefix
+  Form own_form, pre_form;
   PagedPass own, pre;
   int64_t own_units, pre_units;  // per K/V head
   int64_t bytes;
@@ -1134,49 +1178,81 @@ struct Layout {
 
 int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
-constexpr int32_t kWideSlots = 512;
-constexpr int32_t kWideLeast = 4;
-constexpr int32_t kNarrowSlots = 1024;
-constexpr int32_t kNarrowLeast = 4;
+// Units per K/V head of a launch of up to `tiles` tiles of up to `chunks` chunks each.
+int64_t units_bound(const PagedPass& p, int64_t tiles, int64_t chunks) {
+  // total / c for any total up to this one: c >= least, and c >= total / wanted or
+  // else c >= cap and c >= total / most
+  const int64_t total = tiles * chunks;
+  int64_t cuts = total / p.cap < p.most ? total / p.cap : p.most;
+  if (cuts < p.wanted) cuts = p.wanted;
+  if (cuts > total / p.least) cuts = total / p.least;
+  return tiles + cuts;
+}
 
-// A launch of one kind of tile: rows, and the parts that fill the card.
-void shape(PagedPass& p, bool narrow, int32_t kv_heads) {
-  p.rows = narrow ? kNarrowRows : kWideRows;
-  p.least = narrow ? kNarrowLeast : kWideLeast;
-  p.wanted = ((narrow ? kNarrowSlots : kWideSlots) + kv_heads - 1) / kv_heads;
+// How a launch of up to `tiles` tiles (per K/V head) of up to `chunks` chunks runs.
+Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_heads) {
+  p.cap = 0x7fffffff;
+  if (!narrow) {
+    p.least = p.always ? 4 : XWL;
+    p.wanted = p.most = (512 + kv_heads - 1) / kv_heads;
+    return kWide;
+  }
+  if (chunks <= kUncut && tiles * kv_heads <= 256) {
+    p.least = kUncut;
+    p.wanted = p.most = 1;
+    return kNarrowAlone;
+  }
+  p.least = 4;
+  p.cap = 48;
+  const int64_t per_unit = tiles * kv_heads * chunks / 256;
+  const bool longer = chunks >= kLongUnit && per_unit >= kLongUnit;
+  p.wanted = ((longer ? 256 : 512) + kv_heads - 1) / kv_heads;
+  p.most = 4 * p.wanted;
+  return longer ? kNarrowLong : kNarrowMany;
 }
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
-                 int32_t prefix_len, void* workspace) {
+                 int32_t prefix_len, int64_t window, int64_t sinks, void* workspace) {
   Layout l{};
   const int64_t group = heads / kv_heads;
   const int64_t rows = tokens * group;
   const int64_t busy = requests < tokens ? requests : tokens;  // requests with queries
-  l.shared = prefix_len > 0 && rows < 64 * busy;
-  l.narrow = rows <= kNarrowRows * busy && !(prefix_len > 0 && !l.shared);
-  shape(l.own, l.narrow, kv_heads);
+  const int64_t prefix_chunks = (static_cast<int64_t>(prefix_len) + kBN - 1) / kBN;
+  int64_t longest = (table_rows + kBN - 1) / kBN;  // chunks of a tile
+  const int64_t seen = (window + tokens) / kBN + 2 + (sinks + kBN - 1) / kBN;
+  if (window > 0 && seen < longest) longest = seen;
+  bool narrow = rows <= kNarrowRows * busy;
+  // A prefix has a pass of its own where its rows are read by few rows per
+  // request; else it heads each tile's keys.
+  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= XCONCAT);
   l.own.with_prefix = prefix_len > 0 && !l.shared;
+  if (l.own.with_prefix) longest += prefix_chunks;
   l.own.always = l.shared;
-  l.own_units = rows / l.own.rows + busy + l.own.wanted;
-  const int64_t longest = (table_rows + kBN - 1) / kBN + 1 + (l.own.with_prefix ? (prefix_len + kBN - 1) / kBN : 0);
+  l.own.rows = narrow ? kNarrowRows : kWideRows;
+  const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
+  l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
+  l.own_units = l.own_form == kNarrowAlone ? tiles : units_bound(l.own, tiles, longest);
   l.own.combined = l.shared || longest > l.own.least;
   int64_t at = 0;
-  auto place = [&](PagedPass& p, int64_t records) {
+  // records: of tiles that are cut, at most twice the cuts; of all where all are joined
+  auto place = [&](PagedPass& p, int64_t units, int64_t tiles) {
     char* const base = static_cast<char*>(workspace);
+    const int64_t cuts = units - tiles;
     p.records = reinterpret_cast<float*>(base + at);
-    at += round256(records * kv_heads * p.rows * (dim + 2) * 4);
+    at += round256((p.always ? units : 2 * cuts + 1) * kv_heads * p.rows * (dim + 2) * 4);
     p.meta = reinterpret_cast<int2*>(base + at);
     at += round256(rows * 8);
   };
-  if (l.own.combined) place(l.own, 2 * l.own.wanted + 2 + (l.own.always ? rows / l.own.rows + busy : 0));
+  if (l.own.combined) place(l.own, l.own_units, tiles);
   if (l.shared) {
     l.pre = l.own;
     l.pre.shared = 1;
-    l.shared_narrow = rows <= kNarrowRows;
-    shape(l.pre, l.shared_narrow, kv_heads);
+    narrow = rows <= kNarrowRows;
+    l.pre.rows = narrow ? kNarrowRows : kWideRows;
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
-    l.pre_units = tiles + l.pre.wanted;
-    place(l.pre, 2 * l.pre.wanted + 2 + tiles);
+    l.pre_form = shape(l.pre, narrow, tiles, prefix_chunks, kv_heads);
+    l.pre_units = l.pre_form == kNarrowAlone ? tiles : units_bound(l.pre, tiles, prefix_chunks);
+    place(l.pre, l.pre_units, tiles);
   }
   l.bytes = at;
   return l;
@@ -1185,16 +1261,22 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
 template <int DT, int D>
 hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream) {
   const Layout l = layout_of(a.num_tokens, a.requests, a.heads, a.kv_heads, D,
-                             static_cast<int64_t>(a.table_width) << a.block_shift, a.prefix_len, a.workspace);
+                             static_cast<int64_t>(a.table_width) << a.block_shift, a.prefix_len, a.window, a.sinks,
+                             a.workspace);
   const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
-  const auto run = [&](const PagedPass& p, int32_t narrow, int64_t units) {
-    if (narrow) paged_narrow_kernel<DT, D><<<grid(units), 128, 0, stream>>>(a, p, sc);
-    else paged_wide_kernel<DT, D><<<grid(units), 256, 0, stream>>>(a, p, sc);
+  const auto run = [&](const PagedPass& p, Form form, int64_t units) {
+    constexpr int kMore = D == 128 ? 1 : 2;  // rows of 64 are half as long
+    switch (form) {
+      case kWide: paged_wide_kernel<DT, D><<<grid(units), 256, 0, stream>>>(a, p, sc); break;
+      case kNarrowMany: paged_narrow_kernel<DT, D, 2, 2 * kMore><<<grid(units), 128, 0, stream>>>(a, p, sc); break;
+      case kNarrowLong: paged_narrow_kernel<DT, D, 4, 2 * kMore><<<grid(units), 256, 0, stream>>>(a, p, sc); break;
+      case kNarrowAlone: paged_narrow_kernel<DT, D, 8, kMore><<<grid(units), 512, 0, stream>>>(a, p, sc); break;
+    }
   };
-  if (l.shared) run(l.pre, l.shared_narrow, l.pre_units);
-  run(l.own, l.narrow, l.own_units);
+  if (l.shared) run(l.pre, l.pre_form, l.pre_units);
+  run(l.own, l.own_form, l.own_units);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !l.own.combined) return e;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.heads / a.kv_heads);
@@ -1211,8 +1293,8 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
 }  // namespace
 
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                                  int64_t table_rows, int32_t prefix_len) {
-  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, nullptr).bytes;
+                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks) {
+  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, window, sinks, nullptr).bytes;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
