@@ -129,8 +129,9 @@ SIGNATURES = {
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p,
          _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32,
-         _c_i32, _c_i32, ctypes.c_float, _c_i32, _c_p, _c_i64, _c_p],
+         _c_i32, _c_i32, ctypes.c_float, _c_i32, _c_p, _c_i64, _c_p, _c_p],
     ),
+    "hkv_paged_attention_counter_bytes": (_c_i64, []),
 }
 
 
@@ -336,3 +337,37 @@ def attention_workspace(device: torch.device, stream=None):
         ws = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", idx))
         _workspaces[key] = ws
     return ws
+
+
+# Counters of the paged attention (zeroed; every launch leaves them zero), kept
+# like the workspaces above.
+_paged_counters: dict = {}
+_capture_paged_counters: dict = {}
+
+
+def paged_counters(device: torch.device, stream=None) -> torch.Tensor:
+    """Counters of ``hkv_paged_attention`` for the current stream of ``device``
+    (or ``stream``): one buffer per (device, stream), cleared once; under
+    HIP-graph capture one per capture, cleared by a fill kernel that the graph
+    replays before its first use."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if stream is None:
+        stream = torch.cuda.current_stream(idx)
+    key = (idx, stream.cuda_stream)
+    if torch.cuda.is_current_stream_capturing():
+        cid = capture_id(stream.cuda_stream)
+        hit = _capture_paged_counters.get(key)
+        if hit is None or hit[0] != cid:
+            hit = (cid, _new_paged_counters(idx))
+            _capture_paged_counters[key] = hit
+        return hit[1]
+    buf = _paged_counters.get(key)
+    if buf is None:
+        buf = _paged_counters[key] = _new_paged_counters(idx)
+    return buf
+
+
+def _new_paged_counters(idx: int) -> torch.Tensor:
+    need = int(load().hkv_paged_attention_counter_bytes())
+    buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", idx))
+    return buf.zero_()

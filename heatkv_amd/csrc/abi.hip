@@ -797,6 +797,8 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
   return ok();
 }
 
+int64_t hkv_paged_attention_counter_bytes(void) { return hkv::kPagedCounterBytes; }
+
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
                                             int32_t prefix_length, int32_t window, int32_t sinks) {
@@ -821,7 +823,7 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
                             int32_t table_width, int32_t num_blocks, int32_t heads, int32_t kv_heads,
                             int32_t head_dim, int32_t block_size, int32_t window, int32_t sinks, int32_t causal,
                             int32_t dtype, float softmax_scale, int32_t fill_tail, void* workspace,
-                            int64_t workspace_bytes, void* stream) {
+                            int64_t workspace_bytes, void* counters, void* stream) {
   const int32_t shift = block_shift_of(block_size);
   if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
   if (num_tokens < 0 || requests < 0 || table_width < 0 || num_blocks < 0 || window < 0 || sinks < 0 ||
@@ -860,11 +862,14 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256))
     return fail(HKV_ERR_INVALID_ARG, "the call needs %lld bytes of 256-byte aligned workspace",
                 static_cast<long long>(need));
+  if (reinterpret_cast<uintptr_t>(counters) % 64 != 0)
+    return fail(HKV_ERR_INVALID_ARG, "counters must be 64-byte aligned");
   hkv::PagedAttnArgs a{q, q_token_stride, q_head_stride, k_cache, v_cache,
                        {k_block_stride, k_head_stride, k_row_stride}, {v_block_stride, v_head_stride, v_row_stride},
                        block_tables, table_stride, lengths, query_starts, prefix_blocks, prefix_length, out, lse,
                        num_tokens, requests, table_width, num_blocks, heads, kv_heads, head_dim, shift, window, sinks,
-                       causal != 0 ? 1 : 0, dtype, fill_tail != 0 ? 1 : 0, softmax_scale, workspace, workspace_bytes};
+                       causal != 0 ? 1 : 0, dtype, fill_tail != 0 ? 1 : 0, softmax_scale, workspace, workspace_bytes,
+                       static_cast<int32_t*>(counters)};
   const hipError_t e = hkv::launch_paged_attention(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(HKV_ERR_LAUNCH, "paged attention launch failed: %s", hipGetErrorString(e));
   return ok();

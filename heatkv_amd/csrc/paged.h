@@ -84,7 +84,9 @@ struct PagedAttnArgs {
   float softmax_scale;
   void* workspace;
   int64_t workspace_bytes;
+  int32_t* counters;  // zeroed kPagedCounterBytes that every launch leaves zero, or null
 };
+constexpr int64_t kPagedCounterBytes = 64 * 1024;
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                   int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks);

@@ -48,6 +48,7 @@ struct PagedPass {
   int32_t cap;       // chunks of a part from which more than `wanted` are made
   int32_t always;    // every tile leaves records (a shared prefix is joined to it)
   int32_t combined;  // a combine launch follows: write meta
+  int32_t join;      // the last part of a cut tile joins its records (counters)
   float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
   int2* meta;        // per live row: first record, parts | row in tile << 16
 };
@@ -56,10 +57,15 @@ __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_
 
 // Chunks of a part in a launch of `total` chunks (per K/V head): total / c, the
 // number of parts, never falls with total and is at most `most`.
+__host__ __device__ __forceinline__ int64_t up_div(int64_t a, int32_t b) {
+  // 32-bit where that does (64-bit divisions cost about 150 instructions)
+  const int64_t n = a + b - 1;
+  return n >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(b)) : n / b;
+}
 __host__ __device__ __forceinline__ int64_t part_chunks(const PagedPass& p, int64_t total) {
-  int64_t c = (total + p.wanted - 1) / p.wanted;
+  int64_t c = up_div(total, p.wanted);
   if (c > p.cap) {
-    c = (total + p.most - 1) / p.most;
+    c = up_div(total, p.most);
     c = c > p.cap ? c : p.cap;
   }
   return c > p.least ? c : p.least;
@@ -133,7 +139,7 @@ __device__ __forceinline__ Load load_of(const PagedAttnArgs& a, const PagedPass&
   const int32_t group = a.heads / a.kv_heads;
   Load l{0, 0};
   if (g.n == 0) return l;
-  l.tiles = (g.n * group + p.rows - 1) / p.rows;
+  l.tiles = (g.n * group + p.rows - 1) >> (p.rows == kWideRows ? 7 : 4);
   l.chunks = keys_of(a, p, g, 0, g.n - 1).chunks();
   return l;
 }
@@ -145,10 +151,11 @@ struct Work {
   int32_t parts;    // of the request's tiles
   int32_t record;   // of the tile's part 0
   Geometry g;       // of the request
+  int32_t end;      // live tokens
 };
 
 __device__ __forceinline__ int32_t parts_of(const Load& l, int64_t c) {
-  return l.chunks > c ? static_cast<int32_t>((l.chunks + c - 1) / c) : 1;
+  return l.chunks > c ? static_cast<int32_t>(up_div(l.chunks, static_cast<int32_t>(c))) : 1;
 }
 
 // Units, and records, of a request.
@@ -158,16 +165,16 @@ __device__ __forceinline__ int2 units_of(const PagedPass& p, const Load& l, int6
   return int2{units, parts > 1 || p.always ? units : 0};
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// Sum, and prefix sums, of the first n lanes (the others hold zeros).
+__device__ __forceinline__ int64_t wave_sum64(int64_t v, int n = 64) {
+  for (int off = 1; off < n; off <<= 1) v += __shfl_xor(v, off, 64);
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(v)))) |
+                              static_cast<uint64_t>(uniform(static_cast<int32_t>(v >> 32))) << 32);
 }
 
-__device__ __forceinline__ int2 wave_prefix(int2 v) {
+__device__ __forceinline__ int2 wave_prefix(int2 v, int n = 64) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
+  for (int off = 1; off < n; off <<= 1) {
     const int2 o{__shfl_up(v.x, off, 64), __shfl_up(v.y, off, 64)};
     if (lane >= off) v = int2{v.x + o.x, v.y + o.y};
   }
@@ -180,7 +187,7 @@ template <int kThreads>
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
-  Work w{-1, 0, 0, 1, 0, {0, 0, 0}};
+  Work w{-1, 0, 0, 1, 0, {0, 0, 0}, live_tokens(a)};
   if (R <= 64) {
     Load l{0, 0};
     Geometry g{0, 0, 0};
@@ -188,11 +195,11 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
       g = load_request(a, p, lane);
       l = load_of(a, p, g);
     }
-    const int64_t total = wave_sum64(static_cast<int64_t>(l.tiles) * l.chunks);
+    const int64_t total = wave_sum64(static_cast<int64_t>(l.tiles) * l.chunks, R);
     const int64_t c = part_chunks(p, total);
     const int2 mine = units_of(p, l, c);
-    const int2 end = wave_prefix(mine);
-    const uint64_t hit = __ballot(unit >= end.x - mine.x && unit < end.x);
+    const int2 end = wave_prefix(mine, R);
+    const uint64_t hit = __ballot(lane < R && unit >= end.x - mine.x && unit < end.x);
     if (hit == 0) return w;
     const int src = __builtin_ctzll(hit);
     const int32_t parts = __builtin_amdgcn_readlane(parts_of(l, c), src);
@@ -296,8 +303,9 @@ __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPas
   const int32_t most = (n + p.least - 1) / p.least;
   t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
   if (w.part >= t.parts) return false;
-  t.t0 = static_cast<int32_t>(static_cast<int64_t>(n) * w.part / t.parts);
-  t.t1 = static_cast<int32_t>(static_cast<int64_t>(n) * (w.part + 1) / t.parts);
+  const int32_t each = n / t.parts, more = n - each * t.parts;  // the first `more` parts have one chunk more
+  t.t0 = each * w.part + (w.part < more ? w.part : more);
+  t.t1 = t.t0 + each + (w.part < more ? 1 : 0);
   return true;
 }
 
@@ -394,9 +402,7 @@ __device__ __forceinline__ void split_finite(u32x4_t& v, u32x4_t& up, u32x4_t& d
 
 // Zeros (lse -inf) for the tokens behind the last request, shared by all workgroups.
 template <int kThreads>
-__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a) {
-  const int32_t live = live_tokens(a);
-  if (live >= a.num_tokens) return;
+__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t live) {
   const int64_t units = static_cast<int64_t>(a.num_tokens - live) * a.heads * (a.head_dim / 8);
   uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
                                               static_cast<int64_t>(live) * a.heads * a.head_dim);
@@ -452,8 +458,8 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
   const int32_t group = a.heads / a.kv_heads;
   const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
-  if (a.fill_tail && !p.shared) fill_tail<kThreads>(a);
   const Work w = find_work<kThreads>(a, p, unit);
+  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -785,6 +791,90 @@ __device__ __forceinline__ float quad_sum(float v) {
                   __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 
+// 8 bytes of a record, coherent across the XCDs (attn_common.h has the reasons).
+__device__ __forceinline__ f32x2_t ld_agent2(const float* p) {
+  return __builtin_bit_cast(f32x2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// A part of a cut tile has left its record and counts itself in; the last to do so
+// joins all of them in part order, a wave per row, and clears the counter.
+// Nothing waits: a part that is not the last is done.
+template <int DT, int D, int NW>
+__device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const PagedPass& p, const Scalars& sc,
+                                           const Tile& t, const Work& w, int32_t kvh, int32_t& turn) {
+  const int lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6);
+  int32_t* const counter = a.counters + 2 * (static_cast<int64_t>(w.record) * a.kv_heads + kvh);
+  wait_vmcnt<0>();  // every wave's share of the record is written before it is counted
+  __syncthreads();
+  if (threadIdx.x == 0)
+    turn = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == t.parts - 1;
+  __syncthreads();
+  if (!turn) return;
+  constexpr int kLanes = D / 2;         // of a part's row
+  constexpr int kAtOnce = 64 / kLanes;  // parts per load
+  const int32_t group = a.heads / a.kv_heads;
+  const int64_t stride = static_cast<int64_t>(a.kv_heads) * (p.rows * (D + 2));
+  const float* const rec0 = record_of<D>(a, p, w.record, kvh);
+  for (int32_t row = wave; row < t.rows; row += NW) {
+    float top = kNoMax, sum = 0.f;
+    f32x2_t acc{};
+    for (int32_t q0 = 0; q0 < t.parts; q0 += 64) {
+      const int32_t count = t.parts - q0 < 64 ? t.parts - q0 : 64;
+      float pm = kNoMax, pl = 0.f;
+      if (lane < count) {
+        const float* const ml = rec0 + (q0 + lane) * stride + p.rows * D + row;
+        pm = ld_agent(ml);
+        pl = ld_agent(ml + p.rows);
+      }
+      float mn = pm;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) mn = fmaxf(mn, __shfl_xor(mn, off, 64));
+      mn = fmaxf(top, mn);
+      const float x = __builtin_amdgcn_exp2f((top - mn) * sc.c), y = __builtin_amdgcn_exp2f((pm - mn) * sc.c);
+      float add = pl * y;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) add += __shfl_xor(add, off, 64);
+      sum = sum * x + add;
+      top = mn;
+      acc *= x;
+      const float* const o = rec0 + q0 * stride + row * D + (lane % kLanes) * 2;
+#pragma unroll 1
+      for (int32_t base = 0; base < count; base += 8 * kAtOnce) {
+        f32x2_t v[8];
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int32_t mine = base + i * kAtOnce + lane / kLanes;
+          const int32_t at = mine < count ? mine : 0;
+          v[i] = ld_agent2(o + at * stride);
+          z[i] = __shfl(y, at, 64);
+          if (mine >= count) v[i] = f32x2_t{};
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc += v[i] * z[i];
+      }
+    }
+    if constexpr (kAtOnce > 1) {
+      acc[0] += __shfl_xor(acc[0], 32, 64);
+      acc[1] += __shfl_xor(acc[1], 32, 64);
+    }
+    const int32_t mat = t.row0 + row;
+    const int32_t tok = mat / group;
+    const int32_t head = kvh * group + (mat - tok * group);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = static_cast<int64_t>(t.g.first + tok) * a.heads + head;
+    if (lane < kLanes)
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at * D + lane * 2) =
+          pack2<DT>(acc[0] * inv, acc[1] * inv);
+    if (a.lse != nullptr && lane == 0)
+      a.lse[static_cast<int64_t>(head) * a.num_tokens + t.g.first + tok] =
+          sum == 0.f ? -__builtin_inff() : (top * sc.c + __log2f(sum)) * 0.6931471805599453f;
+  }
+  if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 template <int DT, int D, int NW, int NS>
 __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
                                                               const Scalars sc) {
@@ -804,6 +894,7 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
     const uint8_t* rows[2][kKeys];
   };
   __shared__ __attribute__((aligned(1024))) Wave lds_waves[NW];
+  __shared__ int32_t turn;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -813,8 +904,8 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
   const int32_t group = a.heads / a.kv_heads;
   const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
   const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
-  if (a.fill_tail && !p.shared) fill_tail<kThreads>(a);
   const Work w = find_work<kThreads>(a, p, unit);
+  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -1022,44 +1113,65 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
   }
   float l = quad_sum(l_run);
 
-  // the other waves' results join wave 0's, in their order
+  // the waves' results are joined in their order, each wave taking its share of the dimensions
+  constexpr int kMine = (DB + NW - 1) / NW;
   float* const left = reinterpret_cast<float*>(my.ring);
-  if (wave != 0) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(left + (db * 64 + lane) * 4) = oacc[db];
-    left[DB * 256 + lane] = m_run;
-    left[DB * 256 + 64 + lane] = l;
-  }
+  for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(left + (db * 64 + lane) * 4) = oacc[db];
+  left[DB * 256 + lane] = m_run;
+  left[DB * 256 + 64 + lane] = l;
   __syncthreads();
-  if (wave != 0) return;
+  float ms[NW];
+  f32x4_t o[kMine];
 #pragma unroll
-  for (int v = 1; v < NW; ++v) {
-    const float* const other = reinterpret_cast<const float*>(lds_waves[v].ring);
-    const float m1 = other[DB * 256 + lane], l1 = other[DB * 256 + 64 + lane];
-    const float m_new = fmaxf(m_run, m1);
-    const float x = __builtin_amdgcn_exp2f((m_run - m_new) * sc.c), y = __builtin_amdgcn_exp2f((m1 - m_new) * sc.c);
-    l = l * x + l1 * y;
+  for (int i = 0; i < kMine; ++i) o[i] = f32x4_t{};
+  m_run = kNoMax;
+  l = 0.f;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-      oacc[db] = oacc[db] * x + *reinterpret_cast<const f32x4_t*>(other + (db * 64 + lane) * 4) * y;
-    m_run = m_new;
+  for (int v = 0; v < NW; ++v) {
+    ms[v] = reinterpret_cast<const float*>(lds_waves[v].ring)[DB * 256 + lane];
+    m_run = fmaxf(m_run, ms[v]);
   }
-  if (q >= t.rows) return;
+  const int db0 = wave * kMine;
+#pragma unroll
+  for (int v = 0; v < NW; ++v) {
+    const float* const other = reinterpret_cast<const float*>(lds_waves[v].ring);
+    const float y = __builtin_amdgcn_exp2f((ms[v] - m_run) * sc.c);
+    l += other[DB * 256 + 64 + lane] * y;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (db0 + i < DB) o[i] += *reinterpret_cast<const f32x4_t*>(other + ((db0 + i) * 64 + lane) * 4) * y;
+  }
   if (t.parts > 1 || p.always) {
     float* const rec = record_of<D>(a, p, w.record + w.part, kvh);
+    const bool join = t.parts > 1 && p.join;
+    if (q < t.rows) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(rec + q * D + db * 16 + 4 * g) = oacc[db];
-    if (g == 0) {
-      rec[p.rows * D + q] = m_run;
-      rec[p.rows * (D + 1) + q] = l;
+      for (int i = 0; i < kMine; ++i) {
+        if (db0 + i >= DB) break;
+        float* const to = rec + q * D + (db0 + i) * 16 + 4 * g;
+        if (join) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) st_agent(to + k, o[i][k]);
+        } else {
+          *reinterpret_cast<f32x4_t*>(to) = o[i];
+        }
+      }
+      if (wave == 0 && g == 0) {
+        st_agent(rec + p.rows * D + q, m_run);
+        st_agent(rec + p.rows * (D + 1) + q, l);
+      }
     }
+    if (join) join_parts<DT, D, NW>(a, p, sc, t, w, kvh, turn);
     return;
   }
+  if (q >= t.rows) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t at = (static_cast<int64_t>(t.g.first + tok) * a.heads + head) * D + 4 * g;
 #pragma unroll
-  for (int db = 0; db < DB; ++db) store4<DT>(a.out, at + db * 16, oacc[db] * inv);
-  if (a.lse != nullptr && g == 0)
+  for (int i = 0; i < kMine; ++i)
+    if (db0 + i < DB) store4<DT>(a.out, at + (db0 + i) * 16, o[i] * inv);
+  if (a.lse != nullptr && wave == 0 && g == 0)
     a.lse[static_cast<int64_t>(head) * a.num_tokens + t.g.first + tok] =
         l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
 }
@@ -1150,13 +1262,13 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
 #define XWL 8
 #endif
 #ifndef XLONG
-#define XLONG 16
+#define XLONG 32
 #endif
 #ifndef XSHORT
 #define XSHORT 16
 #endif
 #ifndef XCONCAT
-#define XCONCAT 2048
+#define XCONCAT 4096
 #endif
 // What runs a launch's tiles.
 enum Form : int32_t {
@@ -1212,7 +1324,7 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
 }
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
-                 int32_t prefix_len, int64_t window, int64_t sinks, void* workspace) {
+                 int32_t prefix_len, int64_t window, int64_t sinks, void* workspace, bool counters) {
   Layout l{};
   const int64_t group = heads / kv_heads;
   const int64_t rows = tokens * group;
@@ -1232,7 +1344,11 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
   l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
   l.own_units = l.own_form == kNarrowAlone ? tiles : units_bound(l.own, tiles, longest);
-  l.own.combined = l.shared || longest > l.own.least;
+  const bool may_cut = longest > l.own.least;
+  // a record's counter is 8 bytes of the counters
+  l.own.join = counters && may_cut && l.own_form != kWide && !l.shared &&
+               (2 * (l.own_units - tiles) + 1) * kv_heads * 8 <= kPagedCounterBytes;
+  l.own.combined = l.shared || (may_cut && !l.own.join);
   int64_t at = 0;
   // records: of tiles that are cut, at most twice the cuts; of all where all are joined
   auto place = [&](PagedPass& p, int64_t units, int64_t tiles) {
@@ -1243,7 +1359,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     p.meta = reinterpret_cast<int2*>(base + at);
     at += round256(rows * 8);
   };
-  if (l.own.combined) place(l.own, l.own_units, tiles);
+  if (may_cut || l.shared) place(l.own, l.own_units, tiles);
   if (l.shared) {
     l.pre = l.own;
     l.pre.shared = 1;
@@ -1262,7 +1378,7 @@ template <int DT, int D>
 hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream) {
   const Layout l = layout_of(a.num_tokens, a.requests, a.heads, a.kv_heads, D,
                              static_cast<int64_t>(a.table_width) << a.block_shift, a.prefix_len, a.window, a.sinks,
-                             a.workspace);
+                             a.workspace, a.counters != nullptr);
   const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
@@ -1294,7 +1410,8 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
 
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                   int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks) {
-  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, window, sinks, nullptr).bytes;
+  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, window, sinks, nullptr,
+                   false).bytes;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {

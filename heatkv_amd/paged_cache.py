@@ -286,7 +286,8 @@ def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_ta
           prefix_blocks.data_ptr() if prefix_length > 0 else None, prefix_length, out.data_ptr(),
           lse.data_ptr() if lse is not None else None, T, R, M, n, heads, kv_heads, dim, block, window, sinks,
           1 if causal else 0, _lib.dtype_code(q.dtype), float(softmax_scale), 1 if fill else 0,
-          ws.data_ptr() if ws is not None else None, need)
+          ws.data_ptr() if ws is not None else None, need,
+          _lib.paged_counters(device).data_ptr() if need > 0 else None)
     return (out, lse) if return_lse else out
 
 

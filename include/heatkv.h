@@ -494,8 +494,12 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
  * (fill_tail 0) or get the same (fill_tail 1).  Table entries of rows that no
  * query sees are not used.  workspace: hkv_paged_attention_workspace_bytes
  * bytes (0: none needed), 256-byte aligned, contents before and after are of
- * no meaning; calls that can overlap need buffers of their own.
+ * no meaning.  counters: NULL, or hkv_paged_attention_counter_bytes() zeroed
+ * bytes, 64-byte aligned, which every call leaves zero; with them the parts of
+ * a few long rows are joined by the last of them instead of by a second
+ * launch.  Calls that can overlap need buffers of their own for both.
  */
+int64_t hkv_paged_attention_counter_bytes(void);
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
                                             int32_t prefix_length, int32_t window, int32_t sinks);
@@ -508,7 +512,7 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
                             int32_t table_width, int32_t num_blocks, int32_t heads, int32_t kv_heads,
                             int32_t head_dim, int32_t block_size, int32_t window, int32_t sinks, int32_t causal,
                             int32_t dtype, float softmax_scale, int32_t fill_tail, void* workspace,
-                            int64_t workspace_bytes, void* stream);
+                            int64_t workspace_bytes, void* counters, void* stream);
 
 #ifdef __cplusplus
 }

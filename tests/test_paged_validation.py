@@ -131,7 +131,7 @@ def test_abi_refusals_before_any_device_call():
         import ctypes
         return lib.hkv_paged_attention(n, strides, strides, n, n, strides, strides, strides, strides, strides, strides,
                                        n, M, n, n, n, prefix, n, n, T, R, M, N, H, hk, D, block, 0, 0, 1, dtype,
-                                       ctypes.c_float(1.0), 1, n, 0, n)
+                                       ctypes.c_float(1.0), 1, n, 0, n, n)
     assert attn(H=3) == _lib.HKV_ERR_INVALID_ARG
     assert attn(D=96) == _lib.HKV_ERR_UNSUPPORTED
     assert attn(dtype=3) == _lib.HKV_ERR_UNSUPPORTED
