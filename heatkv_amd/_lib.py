@@ -192,7 +192,8 @@ def _load_op_call(lib) -> None:
     if not isinstance(_ENV_DATA, dict):  # pragma: no cover - another platform's os.environ
         return
     names = ("hkv_segmented_attention", "hkv_segmented_attention_split", "hkv_segmented_attention_split_bytes",
-             "hkv_segmented_attention_item_shape", "hkv_qkv_produce", "hkv_pack_segments")
+             "hkv_segmented_attention_item_shape", "hkv_qkv_produce", "hkv_pack_segments", "hkv_paged_tables",
+             "hkv_paged_append", "hkv_paged_attention", "hkv_paged_attention_workspace_bytes")
     # the extension calls plain addresses: it must have been compiled for these prototypes
     code = {_c_i32: "i", _c_i64: "l", ctypes.c_float: "f", _c_p: "p"}
     want = tuple("".join(code[t] for t in (SIGNATURES[n][0], *SIGNATURES[n][1])) for n in names)
@@ -201,7 +202,7 @@ def _load_op_call(lib) -> None:
                       RuntimeWarning, stacklevel=3)
         return
     _op_call.init(tuple(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), _ENV_DATA,
-                  tuple(os.environ.encodekey(n) for n in _OP_KNOBS), _workspaces, _device_ok)
+                  tuple(os.environ.encodekey(n) for n in _OP_KNOBS), _workspaces, _device_ok, _paged_counters)
     op_call = _op_call
 
 

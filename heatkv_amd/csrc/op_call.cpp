@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -48,10 +49,15 @@ struct State {
   decltype(&hkv_segmented_attention_item_shape) item_shape = nullptr;
   decltype(&hkv_qkv_produce) produce = nullptr;
   decltype(&hkv_pack_segments) pack = nullptr;
+  decltype(&hkv_paged_tables) paged_tables = nullptr;
+  decltype(&hkv_paged_append) paged_append = nullptr;
+  decltype(&hkv_paged_attention) paged_attention = nullptr;
+  decltype(&hkv_paged_attention_workspace_bytes) paged_workspace = nullptr;
   PyObject* env = nullptr;
   PyObject* knobs = nullptr;  // tuple of the environment keys that change a launch
   PyObject* workspaces = nullptr;
   PyObject* devices = nullptr;
+  PyObject* paged_counters = nullptr;  // the paged attention's, per (device, stream)
   PyObject* plan_queries = nullptr;  // attribute names of a work plan
   PyObject* plan_shape = nullptr;
   bool ready = false;
@@ -375,6 +381,208 @@ PyObject* pack_call(PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+// ------------------------------------------------------------- paged cache
+
+// int32 vector of n elements on dev.
+bool ints(const at::Tensor& t, int64_t n, int dev) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.get_device() == dev;
+}
+
+// A block table [R, M] with rows side by side or further apart.
+bool table_rows(const at::Tensor& t, int dev) {
+  return t.scalar_type() == at::kInt && t.dim() == 2 && t.get_device() == dev && t.size(0) <= 4096 &&
+         t.size(1) <= 0x7fffffff && (t.size(1) <= 1 || t.stride(1) == 1) &&
+         (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+}
+
+bool power_of_two(int64_t v) { return v > 0 && v <= (1 << 20) && (v & (v - 1)) == 0; }
+
+bool wants_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+
+// Two caches [blocks, kv_heads, block, dim] of one 16-bit type on dev.
+bool caches(const at::Tensor& k, const at::Tensor& v, int dev) {
+  if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || k.get_device() != dev ||
+      v.get_device() != dev || (k.scalar_type() != at::kHalf && k.scalar_type() != at::kBFloat16))
+    return false;
+  return k.size(0) > 0 && k.size(0) <= 0x7fffffff && k.size(1) > 0 && k.size(1) <= 1024 && power_of_two(k.size(2)) &&
+         (k.size(3) == 64 || k.size(3) == 128) && k.stride(3) == 1 && v.stride(3) == 1 && !wants_grad(k) &&
+         !wants_grad(v);
+}
+
+const int32_t* i32(const at::Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : tensors) {
+    PyObject* o = out != nullptr ? THPVariable_Wrap(t) : nullptr;
+    if (o == nullptr) {
+      Py_XDECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i++, o);
+  }
+  return out;
+}
+
+// paged_tables(block_tables, lengths, new_counts, free_blocks, free_range,
+// num_tokens, block_size, window, sinks, in_place): (slot_map, query_starts, lengths,
+// free_range, status)
+PyObject* paged_tables_call(PyObject* const* args, Py_ssize_t n) {
+  if (!g.ready || n != 10 || !no_modes()) Py_RETURN_NONE;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i)
+    if ((t[i] = plain(args[i])) == nullptr) Py_RETURN_NONE;
+  const at::Tensor &tables = *t[0], &lengths = *t[1], &counts = *t[2], &ring = *t[3], &range = *t[4];
+  int64_t tokens, block, window, sinks;
+  bool in_place;
+  void* stream = nullptr;
+  const int dev = current_device(&stream);
+  if (dev < 0 || !whole(args[5], &tokens) || !whole(args[6], &block) || !whole(args[7], &window) ||
+      !whole(args[8], &sinks) || !flag(args[9], &in_place) || !table_rows(tables, dev) || ring.dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t R = tables.size(0), N = ring.size(0);
+  if (!ints(lengths, R, dev) || !ints(counts, R, dev) || !ints(ring, N, dev) || !ints(range, 2, dev) || tokens < 0 ||
+      tokens > 0x7fffffff || N > 0x7fffffff || !power_of_two(block) || window < 0 || window > 0x7fffffff || sinks < 0 ||
+      sinks > 0x7fffffff)
+    Py_RETURN_NONE;
+  const auto options = lengths.options();
+  at::Tensor slots = at::empty({tokens}, options.dtype(at::kLong));
+  at::Tensor starts = at::empty({R + 1}, options);
+  at::Tensor status = at::empty({3}, options);
+  at::Tensor lengths_out = in_place ? lengths : at::empty({R}, options);
+  at::Tensor range_out = in_place ? range : at::empty({2}, options);
+  int32_t code;
+  Py_BEGIN_ALLOW_THREADS
+  code = g.paged_tables(static_cast<int32_t*>(tables.data_ptr()), tables.stride(0), i32(lengths), i32(counts),
+                        static_cast<int32_t*>(ring.data_ptr()), i32(range), static_cast<int32_t>(R),
+                        static_cast<int32_t>(tables.size(1)), static_cast<int32_t>(N), static_cast<int32_t>(tokens),
+                        static_cast<int32_t>(block), static_cast<int32_t>(window), static_cast<int32_t>(sinks),
+                        static_cast<int64_t*>(slots.data_ptr()), static_cast<int32_t*>(starts.data_ptr()),
+                        static_cast<int32_t*>(lengths_out.data_ptr()), static_cast<int32_t*>(range_out.data_ptr()),
+                        static_cast<int32_t*>(status.data_ptr()), stream);
+  Py_END_ALLOW_THREADS
+  if (code != HKV_OK) Py_RETURN_NONE;
+  at::Tensor first = status.narrow(0, 0, 1);
+  if (!in_place) return tuple_of({slots, starts, lengths_out, range_out, first});
+  Ref a(THPVariable_Wrap(slots)), b(THPVariable_Wrap(starts)), c(THPVariable_Wrap(first));
+  if (a.p == nullptr || b.p == nullptr || c.p == nullptr) return nullptr;
+  return PyTuple_Pack(5, a.p, b.p, args[1], args[4], c.p);
+}
+
+// paged_append(k, v, k_cache, v_cache, slot_map): True when the copy was launched
+PyObject* paged_append_call(PyObject* const* args, Py_ssize_t n) {
+  if (!g.ready || n != 5 || !no_modes()) Py_RETURN_NONE;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i)
+    if ((t[i] = plain(args[i])) == nullptr) Py_RETURN_NONE;
+  const at::Tensor &k = *t[0], &v = *t[1], &kc = *t[2], &vc = *t[3], &slots = *t[4];
+  void* stream = nullptr;
+  const int dev = current_device(&stream);
+  if (dev < 0 || !caches(kc, vc, dev) || k.dim() != 3 || v.sizes() != k.sizes() || k.size(0) > 0x7fffffff ||
+      k.size(1) != kc.size(1) || k.size(2) != kc.size(3) || k.scalar_type() != kc.scalar_type() ||
+      v.scalar_type() != kc.scalar_type() || k.get_device() != dev || v.get_device() != dev || k.stride(2) != 1 ||
+      v.stride(2) != 1 || wants_grad(k) || wants_grad(v) || slots.scalar_type() != at::kLong || slots.dim() != 1 ||
+      slots.size(0) != k.size(0) || !slots.is_contiguous() || slots.get_device() != dev)
+    Py_RETURN_NONE;
+  int32_t code;
+  Py_BEGIN_ALLOW_THREADS
+  code = g.paged_append(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), kc.data_ptr(),
+                        vc.data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2), vc.stride(0), vc.stride(1),
+                        vc.stride(2), static_cast<const int64_t*>(slots.data_ptr()),
+                        static_cast<int32_t>(kc.size(0)), static_cast<int32_t>(k.size(0)),
+                        static_cast<int32_t>(kc.size(1)), static_cast<int32_t>(kc.size(3)),
+                        static_cast<int32_t>(kc.size(2)), stream);
+  Py_END_ALLOW_THREADS
+  if (code != HKV_OK) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+}
+
+// paged_attention(q, k_cache, v_cache, prefix_blocks, prefix_length,
+// block_tables, lengths, query_starts, softmax_scale, window, sinks, causal,
+// out, return_lse): out, or (out, lse)
+PyObject* paged_attention_call(PyObject* const* args, Py_ssize_t n) {
+  if (!g.ready || n != 14 || !no_modes()) Py_RETURN_NONE;
+  const int at_index[6] = {0, 1, 2, 5, 6, 7};
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i)
+    if ((t[i] = plain(args[at_index[i]])) == nullptr) Py_RETURN_NONE;
+  const at::Tensor &q = *t[0], &kc = *t[1], &vc = *t[2], &tables = *t[3], &lengths = *t[4], &starts = *t[5];
+  int64_t prefix, window, sinks;
+  double scale;
+  bool causal, with_lse;
+  void* stream = nullptr;
+  const int dev = current_device(&stream);
+  if (dev < 0 || !whole(args[4], &prefix) || !number(args[8], &scale) || !whole(args[9], &window) ||
+      !whole(args[10], &sinks) || !flag(args[11], &causal) || !flag(args[13], &with_lse) || !caches(kc, vc, dev) ||
+      !table_rows(tables, dev))
+    Py_RETURN_NONE;
+  const at::Tensor* pb = nullptr;
+  if (args[3] != Py_None) {
+    if ((pb = plain(args[3])) == nullptr || pb->dim() != 1 || !ints(*pb, pb->size(0), dev)) Py_RETURN_NONE;
+  }
+  const int64_t hk = kc.size(1), block = kc.size(2), D = kc.size(3), R = tables.size(0), M = tables.size(1);
+  if (prefix < 0 || prefix > 0x7fffffff || (prefix > 0 && (pb == nullptr || prefix > pb->size(0) * block)) ||
+      window < 0 || window > 0x7fffffff || sinks < 0 || sinks > 0x7fffffff || q.dim() != 3 || q.size(2) != D ||
+      q.scalar_type() != kc.scalar_type() || q.get_device() != dev || q.size(0) > 0x7fffffff || q.size(1) <= 0 ||
+      q.size(1) > 1024 || q.size(1) % hk != 0 || q.stride(2) != 1 || ((q.stride(0) | q.stride(1)) & 7) != 0 ||
+      wants_grad(q) || !ints(lengths, R, dev) || !ints(starts, R + 1, dev))
+    Py_RETURN_NONE;
+  for (const at::Tensor* x : {&kc, &vc})
+    if (!aligned(*x) || ((x->stride(0) | x->stride(1) | x->stride(2)) & 7) != 0) Py_RETURN_NONE;
+  if (!aligned(q)) Py_RETURN_NONE;
+  const int64_t T = q.size(0), H = q.size(1);
+  at::Tensor out;
+  const bool fill = args[12] == Py_None;
+  if (!fill) {
+    const at::Tensor* o = plain(args[12]);
+    if (o == nullptr || o->dim() != 2 || o->size(0) != T || o->size(1) != H * D ||
+        o->scalar_type() != q.scalar_type() || o->get_device() != dev || !o->is_contiguous() || !aligned(*o))
+      Py_RETURN_NONE;
+    out = *o;
+  }
+  const int32_t i_t = static_cast<int32_t>(T), i_r = static_cast<int32_t>(R), i_h = static_cast<int32_t>(H),
+                i_hk = static_cast<int32_t>(hk), i_d = static_cast<int32_t>(D), i_m = static_cast<int32_t>(M),
+                i_b = static_cast<int32_t>(block), i_p = static_cast<int32_t>(prefix),
+                i_w = static_cast<int32_t>(window), i_s = static_cast<int32_t>(sinks);
+  const int64_t need = g.paged_workspace(i_t, i_r, i_h, i_hk, i_d, i_m, i_b, i_p, i_w, i_s);
+  if (need < 0) Py_RETURN_NONE;
+  at::Tensor counters;
+  if (need > 0) {
+    Ref index(PyLong_FromLong(dev)), handle(PyLong_FromVoidPtr(stream));
+    Ref key(PyTuple_Pack(2, index.p, handle.p));
+    PyObject* const o = key.p != nullptr ? PyDict_GetItem(g.paged_counters, key.p) : nullptr;
+    if (o == nullptr || !THPVariable_Check(o)) Py_RETURN_NONE;
+    counters = THPVariable_Unpack(o);
+  }
+  const auto options = q.options().requires_grad(false);
+  at::Tensor lse, workspace;
+  if (fill) out = at::empty({T, H * D}, options);
+  if (with_lse) lse = at::empty({H, T}, options.dtype(at::kFloat));
+  if (need > 0) workspace = at::empty({need}, options.dtype(at::kByte));
+  int32_t code;
+  Py_BEGIN_ALLOW_THREADS
+  code = g.paged_attention(q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), kc.stride(0),
+                           kc.stride(1), kc.stride(2), vc.stride(0), vc.stride(1), vc.stride(2), i32(tables),
+                           tables.stride(0), i32(lengths), i32(starts), prefix > 0 ? i32(*pb) : nullptr, i_p,
+                           out.data_ptr(), with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, i_t, i_r, i_m,
+                           static_cast<int32_t>(kc.size(0)), i_h, i_hk, i_d, i_b, i_w, i_s, causal ? 1 : 0,
+                           code_of(q.scalar_type()), static_cast<float>(scale), fill ? 1 : 0,
+                           need > 0 ? workspace.data_ptr() : nullptr, need,
+                           need > 0 ? counters.data_ptr() : nullptr, stream);
+  Py_END_ALLOW_THREADS
+  if (code != HKV_OK) Py_RETURN_NONE;
+  if (!fill) {
+    if (!with_lse) {
+      Py_INCREF(args[12]);
+      return args[12];
+    }
+    Ref l(THPVariable_Wrap(lse));
+    return l.p != nullptr ? PyTuple_Pack(2, args[12], l.p) : nullptr;
+  }
+  return with_lse ? tuple_of({out, lse}) : THPVariable_Wrap(out);
+}
+
 // torch's exceptions (out of memory among them) end at this boundary: the
 // Python body then runs and meets them itself.
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
@@ -402,18 +610,21 @@ std::string prototype(R (*)(A...)) {
 
 // prototypes(): those of init's entry points, in its order.
 PyObject* prototypes(PyObject*, PyObject*) {
-  const std::string p[6] = {prototype(g.attention), prototype(g.attention_split), prototype(g.split_bytes),
-                            prototype(g.item_shape), prototype(g.produce), prototype(g.pack)};
-  return Py_BuildValue("(ssssss)", p[0].c_str(), p[1].c_str(), p[2].c_str(), p[3].c_str(), p[4].c_str(),
-                       p[5].c_str());
+  const std::string p[10] = {prototype(g.attention),    prototype(g.attention_split), prototype(g.split_bytes),
+                             prototype(g.item_shape),   prototype(g.produce),         prototype(g.pack),
+                             prototype(g.paged_tables), prototype(g.paged_append),    prototype(g.paged_attention),
+                             prototype(g.paged_workspace)};
+  return Py_BuildValue("(ssssssssss)", p[0].c_str(), p[1].c_str(), p[2].c_str(), p[3].c_str(), p[4].c_str(),
+                       p[5].c_str(), p[6].c_str(), p[7].c_str(), p[8].c_str(), p[9].c_str());
 }
 
-// init(addresses, env, knobs, workspaces, devices)
+// init(addresses, env, knobs, workspaces, devices, paged_counters)
 PyObject* init(PyObject*, PyObject* args) {
-  unsigned long long a[6];
-  PyObject *env, *knobs, *workspaces, *devices;
-  if (!PyArg_ParseTuple(args, "(KKKKKK)O!O!O!O!", a, a + 1, a + 2, a + 3, a + 4, a + 5, &PyDict_Type, &env,
-                        &PyTuple_Type, &knobs, &PyDict_Type, &workspaces, &PyDict_Type, &devices))
+  unsigned long long a[10];
+  PyObject *env, *knobs, *workspaces, *devices, *counters;
+  if (!PyArg_ParseTuple(args, "(KKKKKKKKKK)O!O!O!O!O!", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8,
+                        a + 9, &PyDict_Type, &env, &PyTuple_Type, &knobs, &PyDict_Type, &workspaces, &PyDict_Type,
+                        &devices, &PyDict_Type, &counters))
     return nullptr;
   if (!g.ready) {
     g.attention = reinterpret_cast<decltype(g.attention)>(a[0]);
@@ -422,11 +633,16 @@ PyObject* init(PyObject*, PyObject* args) {
     g.item_shape = reinterpret_cast<decltype(g.item_shape)>(a[3]);
     g.produce = reinterpret_cast<decltype(g.produce)>(a[4]);
     g.pack = reinterpret_cast<decltype(g.pack)>(a[5]);
-    for (PyObject* o : {env, knobs, workspaces, devices}) Py_INCREF(o);
+    g.paged_tables = reinterpret_cast<decltype(g.paged_tables)>(a[6]);
+    g.paged_append = reinterpret_cast<decltype(g.paged_append)>(a[7]);
+    g.paged_attention = reinterpret_cast<decltype(g.paged_attention)>(a[8]);
+    g.paged_workspace = reinterpret_cast<decltype(g.paged_workspace)>(a[9]);
+    for (PyObject* o : {env, knobs, workspaces, devices, counters}) Py_INCREF(o);
     g.env = env;
     g.knobs = knobs;
     g.workspaces = workspaces;
     g.devices = devices;
+    g.paged_counters = counters;
     g.plan_queries = PyUnicode_InternFromString("hkv_queries_per_item");
     g.plan_shape = PyUnicode_InternFromString("hkv_plan_shape");
     g.ready = g.plan_queries != nullptr && g.plan_shape != nullptr;
@@ -441,8 +657,14 @@ PyMethodDef methods[] = {
      "The QKV producer's launch, or None"},
     {"pack", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<pack_call>)), METH_FASTCALL,
      "The slab pack's launch, or None"},
+    {"paged_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<paged_tables_call>)),
+     METH_FASTCALL, "The paged tables' launch, or None"},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<paged_append_call>)),
+     METH_FASTCALL, "The paged append's launch, or None"},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<paged_attention_call>)),
+     METH_FASTCALL, "The paged attention's launch, or None"},
     {"prototypes", prototypes, METH_NOARGS, "The entry points' prototypes as compiled, in init's order"},
-    {"init", init, METH_VARARGS, "init(addresses, env, knobs, workspaces, devices)"},
+    {"init", init, METH_VARARGS, "init(addresses, env, knobs, workspaces, devices, paged_counters)"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_op_call", "Native call path of the operators", -1, methods};

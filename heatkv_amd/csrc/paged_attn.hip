@@ -46,6 +46,8 @@ struct PagedPass {
   int32_t wanted;    // units per K/V head that fill the card once
   int32_t most;      // ... and that parts may make at most
   int32_t cap;       // chunks of a part from which more than `wanted` are made
+  int32_t step;      // parts are multiples of this many chunks
+  int32_t uncut;     // tiles of up to this many chunks are not cut
   int32_t always;    // every tile leaves records (a shared prefix is joined to it)
   int32_t combined;  // a combine launch follows: write meta
   int32_t join;      // the last part of a cut tile joins its records (counters)
@@ -68,7 +70,8 @@ __host__ __device__ __forceinline__ int64_t part_chunks(const PagedPass& p, int6
     c = up_div(total, p.most);
     c = c > p.cap ? c : p.cap;
   }
-  return c > p.least ? c : p.least;
+  c = c > p.least ? c : p.least;
+  return (c + p.step - 1) & ~static_cast<int64_t>(p.step - 1);
 }
 
 struct Geometry {
@@ -154,13 +157,13 @@ struct Work {
   int32_t end;      // live tokens
 };
 
-__device__ __forceinline__ int32_t parts_of(const Load& l, int64_t c) {
-  return l.chunks > c ? static_cast<int32_t>(up_div(l.chunks, static_cast<int32_t>(c))) : 1;
+__device__ __forceinline__ int32_t parts_of(const PagedPass& p, const Load& l, int64_t c) {
+  return l.chunks > c && l.chunks > p.uncut ? static_cast<int32_t>(up_div(l.chunks, static_cast<int32_t>(c))) : 1;
 }
 
 // Units, and records, of a request.
 __device__ __forceinline__ int2 units_of(const PagedPass& p, const Load& l, int64_t c) {
-  const int32_t parts = parts_of(l, c);
+  const int32_t parts = parts_of(p, l, c);
   const int32_t units = l.tiles * parts;
   return int2{units, parts > 1 || p.always ? units : 0};
 }
@@ -202,7 +205,7 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
     const uint64_t hit = __ballot(lane < R && unit >= end.x - mine.x && unit < end.x);
     if (hit == 0) return w;
     const int src = __builtin_ctzll(hit);
-    const int32_t parts = __builtin_amdgcn_readlane(parts_of(l, c), src);
+    const int32_t parts = __builtin_amdgcn_readlane(parts_of(p, l, c), src);
     const int32_t in = uniform(unit - __builtin_amdgcn_readlane(end.x - mine.x, src));
     w.request = src;
     w.parts = parts;
@@ -249,7 +252,7 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
       const Load l = load_of(a, p, g);
       const int2 u = units_of(p, l, c);
       if (unit < at.x + u.x) {
-        const int32_t parts = parts_of(l, c);
+        const int32_t parts = parts_of(p, l, c);
         const int32_t in = unit - at.x;
         found[0] = r;
         found[1] = l.tiles - 1 - in / parts;
@@ -300,7 +303,7 @@ __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPas
   t.blocks = p.shared ? a.prefix_blocks : a.block_tables + w.request * a.table_stride;
   const int32_t n = t.keys.chunks();
   // a tile with fewer chunks than its request's longest is cut in fewer parts
-  const int32_t most = (n + p.least - 1) / p.least;
+  const int32_t most = n > p.uncut ? (n + p.least - 1) / p.least : 1;
   t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
   if (w.part >= t.parts) return false;
   const int32_t each = n / t.parts, more = n - each * t.parts;  // the first `more` parts have one chunk more
@@ -1258,27 +1261,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
 
 // ---------------------------------------------------------------- launch
 
-#ifndef XWL
-#define XWL 8
-#endif
-#ifndef XLONG
-#define XLONG 32
-#endif
-#ifndef XSHORT
-#define XSHORT 16
-#endif
-#ifndef XCONCAT
-#define XCONCAT 4096
-#endif
 // What runs a launch's tiles.
 enum Form : int32_t {
-  kWide,         // paged_wide_kernel, two workgroups per CU
-  kNarrowMany,   // paged_narrow_kernel, 2 waves, two workgroups per CU
-  kNarrowLong,   // ... 4 waves, one per CU
-  kNarrowAlone,  // ... 8 waves with one stage each, one per CU; no tile is cut
+  kWide,        // paged_wide_kernel, two workgroups per CU
+  kNarrowMany,  // paged_narrow_kernel: two waves of two stages, two workgroups per CU
+  kNarrowOne,   // ... eight waves of one stage, one workgroup per CU
 };
-constexpr int32_t kUncut = XSHORT;      // chunks of a tile that kNarrowAlone takes
-constexpr int32_t kLongUnit = XLONG;   // chunks of a unit from which kNarrowLong is taken
 
 struct Layout {
   int32_t shared;  // a pass of its own for the prefix
@@ -1304,23 +1292,27 @@ int64_t units_bound(const PagedPass& p, int64_t tiles, int64_t chunks) {
 // How a launch of up to `tiles` tiles (per K/V head) of up to `chunks` chunks runs.
 Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_heads) {
   p.cap = 0x7fffffff;
+  p.step = 1;
+  p.uncut = 0;
   if (!narrow) {
-    p.least = p.always ? 4 : XWL;
+    p.least = p.always ? 4 : 8;
     p.wanted = p.most = (512 + kv_heads - 1) / kv_heads;
     return kWide;
   }
-  if (chunks <= kUncut && tiles * kv_heads <= 256) {
-    p.least = kUncut;
-    p.wanted = p.most = 1;
-    return kNarrowAlone;
-  }
+  const int64_t per_cu = tiles * kv_heads * chunks / 256;
   p.least = 4;
-  p.cap = 48;
-  const int64_t per_unit = tiles * kv_heads * chunks / 256;
-  const bool longer = chunks >= kLongUnit && per_unit >= kLongUnit;
-  p.wanted = ((longer ? 256 : 512) + kv_heads - 1) / kv_heads;
+  if (per_cu <= 32 && tiles * kv_heads <= 256) {
+    p.step = 4;  // one stage for each wave
+    p.uncut = 16;
+    p.wanted = p.most = (256 + kv_heads - 1) / kv_heads;
+    return kNarrowOne;
+  }
+  const bool one = chunks >= 32 && per_cu >= 32;
+  p.wanted = ((one ? 256 : 512) + kv_heads - 1) / kv_heads;
   p.most = 4 * p.wanted;
-  return longer ? kNarrowLong : kNarrowMany;
+  p.cap = 48;
+  p.step = one ? 4 : 1;
+  return one ? kNarrowOne : kNarrowMany;
 }
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
@@ -1336,15 +1328,15 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   bool narrow = rows <= kNarrowRows * busy;
   // A prefix has a pass of its own where its rows are read by few rows per
   // request; else it heads each tile's keys.
-  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= XCONCAT);
+  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= 4096);
   l.own.with_prefix = prefix_len > 0 && !l.shared;
   if (l.own.with_prefix) longest += prefix_chunks;
   l.own.always = l.shared;
   l.own.rows = narrow ? kNarrowRows : kWideRows;
   const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
   l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
-  l.own_units = l.own_form == kNarrowAlone ? tiles : units_bound(l.own, tiles, longest);
-  const bool may_cut = longest > l.own.least;
+  l.own_units = units_bound(l.own, tiles, longest);
+  const bool may_cut = longest > l.own.least && longest > l.own.uncut;
   // a record's counter is 8 bytes of the counters
   l.own.join = counters && may_cut && l.own_form != kWide && !l.shared &&
                (2 * (l.own_units - tiles) + 1) * kv_heads * 8 <= kPagedCounterBytes;
@@ -1367,7 +1359,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     l.pre.rows = narrow ? kNarrowRows : kWideRows;
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
     l.pre_form = shape(l.pre, narrow, tiles, prefix_chunks, kv_heads);
-    l.pre_units = l.pre_form == kNarrowAlone ? tiles : units_bound(l.pre, tiles, prefix_chunks);
+    l.pre_units = units_bound(l.pre, tiles, prefix_chunks);
     place(l.pre, l.pre_units, tiles);
   }
   l.bytes = at;
@@ -1387,8 +1379,7 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
     switch (form) {
       case kWide: paged_wide_kernel<DT, D><<<grid(units), 256, 0, stream>>>(a, p, sc); break;
       case kNarrowMany: paged_narrow_kernel<DT, D, 2, 2 * kMore><<<grid(units), 128, 0, stream>>>(a, p, sc); break;
-      case kNarrowLong: paged_narrow_kernel<DT, D, 4, 2 * kMore><<<grid(units), 256, 0, stream>>>(a, p, sc); break;
-      case kNarrowAlone: paged_narrow_kernel<DT, D, 8, kMore><<<grid(units), 512, 0, stream>>>(a, p, sc); break;
+      case kNarrowOne: paged_narrow_kernel<DT, D, 8, kMore><<<grid(units), 512, 0, stream>>>(a, p, sc); break;
     }
   };
   if (l.shared) run(l.pre, l.pre_form, l.pre_units);

@@ -152,6 +152,12 @@ def build_paged_tables(
     as before.  Calling it again with the same inputs gives the same results
     (unless ``in_place``).
     """
+    native = _lib.op_call
+    if native is not None:
+        got = native.paged_tables(block_tables, lengths, new_counts, free_blocks, free_range, num_tokens, block_size,
+                                  window, sinks, in_place)
+        if got is not None:
+            return PagedStep._make(got)
     _check_table(block_tables)
     R, M = (int(x) for x in block_tables.shape)
     device = block_tables.device
@@ -198,6 +204,9 @@ def append_paged_kv(
     any block, head and row strides: ``[N, block, kv_heads, D]`` storage is
     passed as ``cache.transpose(1, 2)``.
     """
+    native = _lib.op_call
+    if native is not None and native.paged_append(k, v, k_cache, v_cache, slot_map):
+        return k_cache, v_cache
     n, heads, block, dim = _check_caches("append_paged_kv", k_cache, v_cache)
     for what, t in (("k", k), ("v", v)):
         if t.ndim != 3 or tuple(t.shape[1:]) != (heads, dim) or t.shape[0] != k.shape[0]:
@@ -226,6 +235,12 @@ def append_paged_kv(
 
 def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_tables, lengths, query_starts,
                softmax_scale, window, sinks, causal, out, return_lse):
+    native = _lib.op_call
+    if native is not None:
+        got = native.paged_attention(q, k_cache, v_cache, prefix_blocks, prefix_length, block_tables, lengths,
+                                     query_starts, softmax_scale, window, sinks, causal, out, return_lse)
+        if got is not None:
+            return got
     n, kv_heads, block, dim = _check_caches(name, k_cache, v_cache)
     device = k_cache.device
     if q.ndim != 3 or int(q.shape[2]) != dim:
@@ -269,8 +284,7 @@ def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_ta
     _no_grad(name, q, k_cache, v_cache)
     _lib.require_device(device)
     if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous() if q.data_ptr() % 16 == 0 and not q.is_contiguous() else q.clone(
-            memory_format=torch.contiguous_format)
+        q = q.clone(memory_format=torch.contiguous_format)
     fill = out is None
     if fill:
         out = torch.empty((T, heads * dim), dtype=q.dtype, device=device)
