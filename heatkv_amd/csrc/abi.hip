@@ -856,6 +856,12 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
                          reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out);
   if (strides % 8 != 0 || ptrs % 16 != 0)
     return fail(HKV_ERR_INVALID_ARG, "q, the caches and out must start at, and their rows lie, 16 bytes apart");
+  // 32-bit byte offsets: between blocks, and of a row in its block
+  const int64_t last = (static_cast<int64_t>(1) << shift) - 1;
+  if (k_block_stride < 0 || v_block_stride < 0 || k_row_stride < 0 || v_row_stride < 0 ||
+      k_block_stride > 0x7fffffffLL || v_block_stride > 0x7fffffffLL || k_row_stride > 0x7fffffffLL ||
+      v_row_stride > 0x7fffffffLL || last * k_row_stride > 0x7fffffffLL || last * v_row_stride > 0x7fffffffLL)
+    return fail(HKV_ERR_UNSUPPORTED, "a block, or the distance between two, of 4 GiB or more");
   const int64_t need = hkv_paged_attention_workspace_bytes(num_tokens, requests, heads, kv_heads, head_dim,
                                                            table_width, block_size, prefix_length, window, sinks);
   if (need < 0) return static_cast<int32_t>(need);

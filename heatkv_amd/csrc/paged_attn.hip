@@ -330,8 +330,14 @@ __device__ __forceinline__ int32_t row_to_load(const PagedAttnArgs& a, const Key
   return j;
 }
 
-__device__ __forceinline__ int64_t block_of(const PagedAttnArgs& a, int32_t raw) {
-  return static_cast<uint32_t>(raw) < static_cast<uint32_t>(a.num_blocks) ? raw : 0;
+// Byte offset in the cache of a request's row whose table entry is `id` (an
+// entry outside the cache stands for block 0).  32-bit strides in bytes.
+__device__ __forceinline__ int64_t row_offset(const PagedAttnArgs& a, const PagedCacheStrides& s, int32_t id,
+                                              int32_t row) {
+  const uint32_t b = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_blocks) ? id : 0;
+  const uint32_t r = row & ((1 << a.block_shift) - 1);
+  return static_cast<int64_t>(static_cast<uint64_t>(b) * static_cast<uint32_t>(s.block * 2) +
+                              r * static_cast<uint32_t>(s.row * 2));
 }
 
 // What a query (row of the matrix) sees of its request's own rows.
@@ -452,6 +458,7 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
   constexpr int kTensor = kBN * D * 2;     // bytes of a chunk's K or V
   constexpr int kStage = 2 * kTensor;
   constexpr int kPitch = D * 2 + 16;
+  __shared__ const uint8_t* v_rows[2][32];
   __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kStage < 4 * 32 * kPitch ? 4 * 32 * kPitch : 2 * kStage];
 
   const int tid = threadIdx.x;
@@ -488,45 +495,37 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
   float m_run = kNoMax, l_run = 0.f;
 
   if (t.t0 < t.t1) {
-    // Rows of this wave in a chunk: [32 half, + 32).  K lanes hold one row (key
-    // lane % 32), V lanes four (key 8 i + 4 (lp / 16) + (lp % 8) / 2).
+    // Rows of this wave in a chunk: [32 half, + 32), a row's address per lane.  K
+    // lanes load their own row, V lanes rows 8 i + 4 (lp / 16) + (lp % 8) / 2, i < 4.
     const bool k_wave = wave < 2;
     const int half = wave & 1;
     const int lp = lane & 31;
-    const int key0 = 32 * half + (k_wave ? lp : 4 * (lp >> 4) + ((lp & 7) >> 1));
+    const int v_row = 4 * (lp >> 4) + ((lp & 7) >> 1);
     const int col = k_wave ? 16 * g : 2 * (32 * g + 16 * ((lp >> 3) & 1) + 8 * (lp & 1));
     const PagedCacheStrides cs = k_wave ? a.ks : a.vs;
-    const uint8_t* const cache =
-        static_cast<const uint8_t*>(k_wave ? a.k_cache : a.v_cache) + kvh * cs.head * 2 + col;
+    const uint8_t* const cache = static_cast<const uint8_t*>(k_wave ? a.k_cache : a.v_cache) + kvh * cs.head * 2;
     const uint32_t lds = lds_address(ring) + (k_wave ? half * (KS * 1024) : kTensor + half * (4 * NP * 1024));
-    const int32_t mask = (1 << a.block_shift) - 1;
-    int32_t rows[4], ids[4];
-    // table entries of the chunk at stream position c
+    int32_t my_row = 0, my_id = 0;
+    // the table entry of this lane's row of the chunk at stream position c
     auto look_up = [&](int32_t c) {
       bool prefix;
-      const int32_t j0 = chunk_row(t.keys, c, prefix) + key0;
-      const int32_t* const blocks = prefix ? a.prefix_blocks : t.blocks;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i > 0 && k_wave) break;
-        rows[i] = row_to_load(a, t.keys, j0 + 8 * i, prefix);
-        ids[i] = blocks[rows[i] >> a.block_shift];
-      }
+      const int32_t j0 = chunk_row(t.keys, c, prefix) + 32 * half;
+      my_row = row_to_load(a, t.keys, j0 + lp, prefix);
+      my_id = (prefix ? a.prefix_blocks : t.blocks)[my_row >> a.block_shift];
     };
-    auto pointer = [&](int i) {
-      return cache + (block_of(a, ids[i]) * cs.block + static_cast<int64_t>(rows[i] & mask) * cs.row) * 2;
-    };
-    // the chunk whose entries were looked up, into stage c % 2
+    // the chunk that was looked up, into stage c % 2
     auto issue = [&](int32_t c) {
       const uint32_t dst = lds + (c & 1) * kStage;
+      const uint8_t* const mine = cache + row_offset(a, cs, my_id, my_row);
       if (k_wave) {
-        const uint8_t* const src = pointer(0);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) dma16(src + 32 * ks, dst + 1024 * ks);
+        for (int ks = 0; ks < KS; ++ks) dma16(mine + col + 32 * ks, dst + 1024 * ks);
       } else {
+        v_rows[half][lp] = mine;
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS operations run in order
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* const src = pointer(i);
+          const uint8_t* const src = v_rows[half][8 * i + v_row] + col;
 #pragma unroll
           for (int n = 0; n < NP; ++n) dma16(src + 128 * n, dst + 1024 * (i * NP + n));
         }
@@ -922,7 +921,6 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
 
   Wave& my = lds_waves[wave];
   const uint32_t ring_lds = lds_address(my.ring);
-  const int32_t mask = (1 << a.block_shift) - 1;
   // the part's 32-key halves of chunks are dealt to the waves in turn
   const int32_t n = (2 * (t.t1 - t.t0) - wave + NW - 1) / NW;
   const auto stage_row = [&](int32_t k, bool& prefix) {
@@ -936,15 +934,15 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
     dma4((prefix ? a.prefix_blocks : t.blocks) + (row_to_load(a, t.keys, j, prefix) >> a.block_shift), lds_address(my.ids[k % NS]));
   };
   const bool for_k = lane < 32;
-  const int64_t block_stride = for_k ? a.ks.block : a.vs.block;
-  const int64_t row_stride = for_k ? a.ks.row : a.vs.row;
+  PagedCacheStrides cs;
+  cs.block = for_k ? a.ks.block : a.vs.block;
+  cs.row = for_k ? a.ks.row : a.vs.row;
   const uint8_t* const cache = static_cast<const uint8_t*>(for_k ? a.k_cache : a.v_cache) +
                                kvh * (for_k ? a.ks.head : a.vs.head) * 2;
   auto issue = [&](int32_t k) {
     bool prefix;
     const int32_t r = row_to_load(a, t.keys, stage_row(k, prefix) + (lane & 31), prefix);
-    const int64_t b = block_of(a, my.ids[k % NS][lane]);
-    my.rows[lane >> 5][lane & 31] = cache + (b * block_stride + static_cast<int64_t>(r & mask) * row_stride) * 2;
+    my.rows[lane >> 5][lane & 31] = cache + row_offset(a, cs, my.ids[k % NS][lane], r);
     const uint32_t dst = ring_lds + (k % NS) * kStage;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -1295,8 +1293,12 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
   p.step = 1;
   p.uncut = 0;
   if (!narrow) {
-    p.least = p.always ? 4 : 8;
-    p.wanted = p.most = (512 + kv_heads - 1) / kv_heads;
+    const bool few = tiles * kv_heads < 256;
+    p.least = few || p.always ? 4 : 8;
+    p.uncut = p.always ? 0 : (few ? 8 : 32);
+    p.wanted = (256 + kv_heads - 1) / kv_heads;
+    p.most = 2 * p.wanted;
+    p.cap = 12;
     return kWide;
   }
   const int64_t per_cu = tiles * kv_heads * chunks / 256;
