@@ -786,6 +786,9 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
     return fail(HKV_ERR_INVALID_ARG, "negative size or no K/V heads");
   if (head_dim != 64 && head_dim != 128)
     return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes head_dim 64 or 128 (got %d)", head_dim);
+  // a thread per 16 bytes (2 where the strides ask for it) and fewer than 2^32 of them
+  if (static_cast<int64_t>(num_tokens) * kv_heads > 0xffffffffLL / head_dim)
+    return fail(HKV_ERR_UNSUPPORTED, "num_tokens * kv_heads * head_dim must be below 2^32");
   if (num_tokens == 0 || num_blocks == 0) return ok();
   if (!k || !v || !k_cache || !v_cache || !slot_map) return fail(HKV_ERR_INVALID_ARG, "null pointer argument");
   hkv::PagedAppendArgs a{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, k_cache, v_cache,

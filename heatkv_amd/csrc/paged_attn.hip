@@ -411,12 +411,12 @@ __device__ __forceinline__ void split_finite(u32x4_t& v, u32x4_t& up, u32x4_t& d
 
 // Zeros (lse -inf) for the tokens behind the last request, shared by all workgroups.
 template <int kThreads>
-__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t live) {
+__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t live, int32_t block, int32_t blocks) {
   const int64_t units = static_cast<int64_t>(a.num_tokens - live) * a.heads * (a.head_dim / 8);
   uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
                                               static_cast<int64_t>(live) * a.heads * a.head_dim);
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t at = static_cast<int64_t>(block) * kThreads + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(blocks) * kThreads;
   for (int64_t i = at; i < units; i += step) out[i] = uint4{0, 0, 0, 0};
   if (a.lse == nullptr) return;
   const int32_t tail = a.num_tokens - live;
@@ -448,28 +448,38 @@ __device__ __forceinline__ void write_meta(const PagedAttnArgs& a, const PagedPa
 // iteration t runs S(t + 1) on the matrix cores beside the exponentials of S(t).
 // Waves 0 and 1 load the K rows, 2 and 3 the V rows, each lane the rows of its
 // own; the table entries of the next chunk are read one iteration ahead.
+template <int D>
+struct WideLds {
+  static constexpr int kTensor = kBN * D * 2;  // bytes of a chunk's K or V
+  static constexpr int kStage = 2 * kTensor;
+  static constexpr int kPitch = D * 2 + 16;    // of a row of the output
+  uint8_t ring[2 * kStage < 4 * 32 * kPitch ? 4 * 32 * kPitch : 2 * kStage];
+  const uint8_t* v_rows[2][32];
+};
+
+// Workgroup `block` of `blocks`.
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs a, const PagedPass p,
-                                                            const Scalars sc) {
+__device__ __forceinline__ void wide_tile(const PagedAttnArgs& a, const PagedPass& p, const Scalars& sc,
+                                          int32_t block, int32_t blocks, WideLds<D>& lds_wide) {
   constexpr int kThreads = 256;
   constexpr int KS = D / 16;               // k-steps of S
   constexpr int DB = D / 32;               // 32-wide blocks of O
   constexpr int NP = D / 64;               // V DMAs per 8 rows
-  constexpr int kTensor = kBN * D * 2;     // bytes of a chunk's K or V
-  constexpr int kStage = 2 * kTensor;
-  constexpr int kPitch = D * 2 + 16;
-  __shared__ const uint8_t* v_rows[2][32];
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kStage < 4 * 32 * kPitch ? 4 * 32 * kPitch : 2 * kStage];
+  constexpr int kTensor = WideLds<D>::kTensor;
+  constexpr int kStage = WideLds<D>::kStage;
+  constexpr int kPitch = WideLds<D>::kPitch;
+  uint8_t* const ring = lds_wide.ring;
+  auto& v_rows = lds_wide.v_rows;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5;
   const int32_t group = a.heads / a.kv_heads;
-  const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
-  const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
+  const int32_t unit = block / a.kv_heads;
+  const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
-  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end);
+  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end, block, blocks);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -758,6 +768,13 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
         l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
 }
 
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                            const Scalars sc) {
+  __shared__ __attribute__((aligned(1024))) WideLds<D> lds;
+  wide_tile<DT, D>(a, p, sc, static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), lds);
+}
+
 // ---------------------------------------------------------------- narrow tiles
 //
 // 16 rows on the 16x16x32 MFMAs; bound by the bytes of the cache.  Two waves, each
@@ -877,9 +894,19 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const PagedPa
   if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A wave's LDS: NS stages of 32 rows of K and V, their table entries, row addresses.
+template <int D, int NS>
+struct NarrowLds {
+  uint8_t ring[NS * 2 * 32 * D * 2];
+  int32_t ids[NS][64];
+  const uint8_t* rows[2][32];
+};
+
+// Workgroup `block` of `blocks`.
 template <int DT, int D, int NW, int NS>
-__global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
-                                                              const Scalars sc) {
+__device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedPass& p, const Scalars& sc,
+                                            int32_t block, int32_t blocks, NarrowLds<D, NS> (&lds_waves)[NW],
+                                            int32_t& turn) {
   constexpr int kThreads = NW * 64;
   constexpr int kKeys = 32;                // of a stage
   constexpr int kRow = D * 2;              // bytes
@@ -890,24 +917,16 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
   constexpr int KS = D / 32;               // k-steps of S
   constexpr int DB = D / 16;               // 16-wide blocks of O
   constexpr int kPieces = D / 8;           // 16-byte pieces of a row
-  struct Wave {
-    uint8_t ring[NS * kStage];
-    int32_t ids[NS][64];
-    const uint8_t* rows[2][kKeys];
-  };
-  __shared__ __attribute__((aligned(1024))) Wave lds_waves[NW];
-  __shared__ int32_t turn;
-
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int q = lane & 15;
   const int g = lane >> 4;
   const int32_t group = a.heads / a.kv_heads;
-  const int32_t unit = static_cast<int32_t>(blockIdx.x) / a.kv_heads;
-  const int32_t kvh = static_cast<int32_t>(blockIdx.x) - unit * a.kv_heads;
+  const int32_t unit = block / a.kv_heads;
+  const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
-  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end);
+  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end, block, blocks);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -919,7 +938,7 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
   const Sight first = sight_of(a, p, t.g, t.row0 / group);
   const Sight last = sight_of(a, p, t.g, (t.row0 + t.rows - 1) / group);
 
-  Wave& my = lds_waves[wave];
+  NarrowLds<D, NS>& my = lds_waves[wave];
   const uint32_t ring_lds = lds_address(my.ring);
   // the part's 32-key halves of chunks are dealt to the waves in turn
   const int32_t n = (2 * (t.t1 - t.t0) - wave + NW - 1) / NW;
@@ -1177,6 +1196,54 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
         l == 0.f ? -__builtin_inff() : (m_run * sc.c + __log2f(l)) * 0.6931471805599453f;
 }
 
+template <int DT, int D, int NW, int NS>
+__global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                              const Scalars sc) {
+  __shared__ __attribute__((aligned(1024))) NarrowLds<D, NS> lds[NW];
+  __shared__ int32_t turn;
+  narrow_tile<DT, D, NW, NS>(a, p, sc, static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), lds, turn);
+}
+
+// ---------------------------------------------------------------- prefix and own rows
+//
+// The prefix's tiles (wide: bound by the matrix cores) and the requests' own (narrow:
+// bound by bytes) in one launch, so that each CU runs one of either.  Workgroups go
+// to the 8 XCDs in turn and to an XCD's 32 CUs in turn, twice: the kinds alternate
+// from CU to CU, and the other way round for a CU's second workgroup.
+template <int DT, int D, bool WIDE>
+__global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a, const PagedPass pre,
+                                                              const PagedPass own, const Scalars sc,
+                                                              const int32_t pre_blocks, const int32_t own_blocks) {
+  constexpr int NW = 4, NS = D == 128 ? 1 : 2;
+  union Lds {
+    WideLds<D> wide;
+    NarrowLds<D, NS> narrow[NW];
+  };
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[sizeof(Lds)];
+  __shared__ int32_t turn;
+  // the id-th workgroup of its kind: of 16 neighbours 8 are the prefix's, while both kinds last
+  const int32_t both = (pre_blocks < own_blocks ? pre_blocks : own_blocks) / 256 * 256;
+  const int32_t b = static_cast<int32_t>(blockIdx.x);
+  bool prefix;
+  int32_t id;
+  if (b < 2 * both) {
+    const int32_t j = b >> 3;  // place in its XCD
+    prefix = ((j + (j >> 5)) & 1) == 0;
+    id = (j >> 1) * 8 + (b & 7);
+  } else {
+    id = b - 2 * both + both;
+    prefix = id < pre_blocks;
+    if (!prefix) id -= pre_blocks - both;
+  }
+  if (prefix) {
+    if constexpr (WIDE) wide_tile<DT, D>(a, pre, sc, id, pre_blocks, *reinterpret_cast<WideLds<D>*>(lds));
+    else
+      narrow_tile<DT, D, NW, NS>(a, pre, sc, id, pre_blocks, *reinterpret_cast<NarrowLds<D, NS>(*)[NW]>(lds), turn);
+  } else {
+    narrow_tile<DT, D, NW, NS>(a, own, sc, id, own_blocks, *reinterpret_cast<NarrowLds<D, NS>(*)[NW]>(lds), turn);
+  }
+}
+
 // ---------------------------------------------------------------- combine
 
 // Joins the records of one row and K/V head: a wave per row.  Up to 64 parts at
@@ -1267,7 +1334,8 @@ enum Form : int32_t {
 };
 
 struct Layout {
-  int32_t shared;  // a pass of its own for the prefix
+  int32_t shared;    // a pass of its own for the prefix ...
+  int32_t together;  // ... in one launch with narrow tiles of the requests' own rows
   Form own_form, pre_form;
   PagedPass own, pre;
   int64_t own_units, pre_units;  // per K/V head
@@ -1361,6 +1429,11 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     l.pre.rows = narrow ? kNarrowRows : kWideRows;
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
     l.pre_form = shape(l.pre, narrow, tiles, prefix_chunks, kv_heads);
+    l.together = l.own_form != kWide;
+    if (l.together && l.pre_form == kWide) {  // one per CU beside the requests' own tiles
+      l.pre.wanted = l.pre.most = (256 + kv_heads - 1) / kv_heads;
+      l.pre.cap = 0x7fffffff;
+    }
     l.pre_units = units_bound(l.pre, tiles, prefix_chunks);
     place(l.pre, l.pre_units, tiles);
   }
@@ -1384,8 +1457,17 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
       case kNarrowOne: paged_narrow_kernel<DT, D, 8, kMore><<<grid(units), 512, 0, stream>>>(a, p, sc); break;
     }
   };
-  if (l.shared) run(l.pre, l.pre_form, l.pre_units);
-  run(l.own, l.own_form, l.own_units);
+  if (l.together) {
+    const int64_t pre = l.pre_units * a.kv_heads, own = l.own_units * a.kv_heads;
+    if (pre + own > 0x7fffffffLL / 256) return hipErrorInvalidConfiguration;
+    const dim3 all(static_cast<uint32_t>(pre + own));
+    const int32_t p = static_cast<int32_t>(pre), o = static_cast<int32_t>(own);
+    if (l.pre_form == kWide) paged_prefix_kernel<DT, D, true><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
+    else paged_prefix_kernel<DT, D, false><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
+  } else {
+    if (l.shared) run(l.pre, l.pre_form, l.pre_units);
+    run(l.own, l.own_form, l.own_units);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !l.own.combined) return e;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.heads / a.kv_heads);
