@@ -816,21 +816,30 @@ __device__ __forceinline__ f32x2_t ld_agent2(const float* p) {
                                                        __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// A part of a cut tile has left its record and counts itself in; the last to do so
-// joins all of them in part order, a wave per row, and clears the counter.
-// Nothing waits: a part that is not the last is done.
+// Counts in a part of a cut tile, whose record every wave has written its share of;
+// true, in all waves, for the last one to do so.  Nothing waits: a part that is not
+// the last is done.
+__device__ __forceinline__ bool last_part(const PagedAttnArgs& a, const Tile& t, const Work& w, int32_t kvh,
+                                          int32_t& turn) {
+  int32_t* const counter = a.counters + 2 * (static_cast<int64_t>(w.record) * a.kv_heads + kvh);
+  wait_vmcnt<0>();  // the record is written before it is counted
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last =
+        __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == t.parts - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    turn = last;
+  }
+  __syncthreads();
+  return turn != 0;
+}
+
+// The last part of a cut tile joins the records of all in part order, a wave per row.
 template <int DT, int D, int NW>
 __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const PagedPass& p, const Scalars& sc,
-                                           const Tile& t, const Work& w, int32_t kvh, int32_t& turn) {
+                                           const Tile& t, const Work& w, int32_t kvh) {
   const int lane = threadIdx.x & 63;
   const int wave = uniform(threadIdx.x >> 6);
-  int32_t* const counter = a.counters + 2 * (static_cast<int64_t>(w.record) * a.kv_heads + kvh);
-  wait_vmcnt<0>();  // every wave's share of the record is written before it is counted
-  __syncthreads();
-  if (threadIdx.x == 0)
-    turn = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == t.parts - 1;
-  __syncthreads();
-  if (!turn) return;
   constexpr int kLanes = D / 2;         // of a part's row
   constexpr int kAtOnce = 64 / kLanes;  // parts per load
   const int32_t group = a.heads / a.kv_heads;
@@ -891,7 +900,6 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const PagedPa
       a.lse[static_cast<int64_t>(head) * a.num_tokens + t.g.first + tok] =
           sum == 0.f ? -__builtin_inff() : (top * sc.c + __log2f(sum)) * 0.6931471805599453f;
   }
-  if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // A wave's LDS: NS stages of 32 rows of K and V, their table entries, row addresses.
@@ -1182,7 +1190,7 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
         st_agent(rec + p.rows * (D + 1) + q, l);
       }
     }
-    if (join) join_parts<DT, D, NW>(a, p, sc, t, w, kvh, turn);
+    if (join && last_part(a, t, w, kvh, turn)) join_parts<DT, D, NW>(a, p, sc, t, w, kvh);
     return;
   }
   if (q >= t.rows) return;
@@ -1363,7 +1371,7 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
   if (!narrow) {
     const bool few = tiles * kv_heads < 256;
     p.least = few || p.always ? 4 : 8;
-    p.uncut = p.always ? 0 : (few ? 8 : 32);
+    p.uncut = p.always ? 0 : (few ? 16 : 32);
     p.wanted = (256 + kv_heads - 1) / kv_heads;
     p.most = 2 * p.wanted;
     p.cap = 12;
@@ -1382,6 +1390,7 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
   p.most = 4 * p.wanted;
   p.cap = 48;
   p.step = one ? 4 : 1;
+  p.uncut = one ? 0 : 16;
   return one ? kNarrowOne : kNarrowMany;
 }
 
@@ -1398,7 +1407,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   bool narrow = rows <= kNarrowRows * busy;
   // A prefix has a pass of its own where its rows are read by few rows per
   // request; else it heads each tile's keys.
-  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= 4096);
+  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= 2048);
   l.own.with_prefix = prefix_len > 0 && !l.shared;
   if (l.own.with_prefix) longest += prefix_chunks;
   l.own.always = l.shared;
