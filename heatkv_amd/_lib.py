@@ -124,7 +124,7 @@ SIGNATURES = {
          _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p],
     ),
     "hkv_paged_attention_workspace_bytes": (
-        _c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+        _c_i64, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "hkv_paged_attention": (
         _c_i32,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p,

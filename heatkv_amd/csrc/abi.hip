@@ -804,7 +804,8 @@ int64_t hkv_paged_attention_counter_bytes(void) { return hkv::kPagedCounterBytes
 
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
-                                            int32_t prefix_length, int32_t window, int32_t sinks) {
+                                            int32_t prefix_length, int32_t window, int32_t sinks,
+                                            int32_t causal) {
   const int32_t shift = block_shift_of(block_size);
   if (shift < 0) return fail(HKV_ERR_INVALID_ARG, "block_size must be a power of two up to 2^20 (got %d)", block_size);
   if (num_tokens < 0 || requests < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 || table_width < 0 ||
@@ -814,7 +815,7 @@ int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests
   return num_tokens == 0 ? 0
                          : hkv::paged_attention_workspace(num_tokens, requests, heads, kv_heads, head_dim,
                                                           static_cast<int64_t>(table_width) << shift, prefix_length, window,
-                                                          sinks);
+                                                          sinks, causal != 0);
 }
 
 int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
@@ -866,7 +867,7 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
       v_row_stride > 0x7fffffffLL || last * k_row_stride > 0x7fffffffLL || last * v_row_stride > 0x7fffffffLL)
     return fail(HKV_ERR_UNSUPPORTED, "a block, or the distance between two, of 4 GiB or more");
   const int64_t need = hkv_paged_attention_workspace_bytes(num_tokens, requests, heads, kv_heads, head_dim,
-                                                           table_width, block_size, prefix_length, window, sinks);
+                                                           table_width, block_size, prefix_length, window, sinks, causal);
   if (need < 0) return static_cast<int32_t>(need);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256))
     return fail(HKV_ERR_INVALID_ARG, "the call needs %lld bytes of 256-byte aligned workspace",

@@ -545,7 +545,7 @@ PyObject* paged_attention_call(PyObject* const* args, Py_ssize_t n) {
                 i_hk = static_cast<int32_t>(hk), i_d = static_cast<int32_t>(D), i_m = static_cast<int32_t>(M),
                 i_b = static_cast<int32_t>(block), i_p = static_cast<int32_t>(prefix),
                 i_w = static_cast<int32_t>(window), i_s = static_cast<int32_t>(sinks);
-  const int64_t need = g.paged_workspace(i_t, i_r, i_h, i_hk, i_d, i_m, i_b, i_p, i_w, i_s);
+  const int64_t need = g.paged_workspace(i_t, i_r, i_h, i_hk, i_d, i_m, i_b, i_p, i_w, i_s, causal ? 1 : 0);
   if (need < 0) Py_RETURN_NONE;
   at::Tensor counters;
   if (need > 0) {

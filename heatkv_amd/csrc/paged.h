@@ -89,6 +89,6 @@ struct PagedAttnArgs {
 constexpr int64_t kPagedCounterBytes = 64 * 1024;
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks);
+                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks, bool causal);
 
 }  // namespace hkv

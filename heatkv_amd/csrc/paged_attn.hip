@@ -42,6 +42,7 @@ struct PagedPass {
   int32_t shared;    // one pseudo request: all live tokens, the prefix's keys
   int32_t with_prefix;  // each tile's keys begin with the prefix (wide tiles that need no sharing)
   int32_t rows;      // rows of a tile
+  int32_t tile_tokens;  // tokens that a tile spans at most
   int32_t least;     // chunks of a part at least
   int32_t wanted;    // units per K/V head that fill the card once
   int32_t most;      // ... and that parts may make at most
@@ -52,6 +53,7 @@ struct PagedPass {
   int32_t combined;  // a combine launch follows: write meta
   int32_t join;      // the last part of a cut tile joins its records (counters)
   float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
+  int32_t limit;     // records there is room for (reached only by query_starts that are not ascending)
   int2* meta;        // per live row: first record, parts | row in tile << 16
 };
 
@@ -86,6 +88,11 @@ __device__ __forceinline__ int32_t clamp32(int32_t v, int32_t lo, int32_t hi) {
 
 __device__ __forceinline__ int32_t live_tokens(const PagedAttnArgs& a) {
   return a.requests > 0 ? clamp32(a.query_starts[a.requests], 0, a.num_tokens) : 0;
+}
+
+// Tokens before the first request (none, as a rule).
+__device__ __forceinline__ int32_t first_token(const PagedAttnArgs& a) {
+  return clamp32(a.query_starts[0], 0, a.num_tokens);
 }
 
 __device__ __forceinline__ Geometry load_request(const PagedAttnArgs& a, const PagedPass& p, int32_t r) {
@@ -135,7 +142,7 @@ __device__ __forceinline__ Keys keys_of(const PagedAttnArgs& a, const PagedPass&
 }
 
 struct Load {
-  int32_t tiles, chunks;  // of a request: tiles of rows, chunks of the longest tile
+  int32_t tiles, chunks;  // of a request: tiles of rows, chunks of a longest tile
 };
 
 __device__ __forceinline__ Load load_of(const PagedAttnArgs& a, const PagedPass& p, const Geometry& g) {
@@ -143,7 +150,10 @@ __device__ __forceinline__ Load load_of(const PagedAttnArgs& a, const PagedPass&
   Load l{0, 0};
   if (g.n == 0) return l;
   l.tiles = (g.n * group + p.rows - 1) >> (p.rows == kWideRows ? 7 : 4);
-  l.chunks = keys_of(a, p, g, 0, g.n - 1).chunks();
+  // causal: the last tile's, else the first's
+  const int32_t span = g.n < p.tile_tokens ? g.n : p.tile_tokens;
+  const int32_t i0 = a.causal && !p.shared ? g.n - span : 0;
+  l.chunks = keys_of(a, p, g, i0, i0 + span - 1).chunks();
   return l;
 }
 
@@ -154,11 +164,14 @@ struct Work {
   int32_t parts;    // of the request's tiles
   int32_t record;   // of the tile's part 0
   Geometry g;       // of the request
-  int32_t end;      // live tokens
+  int32_t head, end;  // the requests' tokens
 };
 
 __device__ __forceinline__ int32_t parts_of(const PagedPass& p, const Load& l, int64_t c) {
-  return l.chunks > c && l.chunks > p.uncut ? static_cast<int32_t>(up_div(l.chunks, static_cast<int32_t>(c))) : 1;
+  if (l.chunks <= c || l.chunks <= p.uncut) return 1;
+  // wide tiles: to the nearest, so that a little over one round is not two
+  if (p.rows == kWideRows) return (l.chunks + static_cast<int32_t>(c) / 2) / static_cast<int32_t>(c);
+  return static_cast<int32_t>(up_div(l.chunks, static_cast<int32_t>(c)));
 }
 
 // Units, and records, of a request.
@@ -190,7 +203,8 @@ template <int kThreads>
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
-  Work w{-1, 0, 0, 1, 0, {0, 0, 0}, live_tokens(a)};
+  Work w{-1, 0, 0, 1, 0, {0, 0, 0}, first_token(a), live_tokens(a)};
+  if (w.end < w.head) w.end = w.head;
   if (R <= 64) {
     Load l{0, 0};
     Geometry g{0, 0, 0};
@@ -305,6 +319,10 @@ __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPas
   // a tile with fewer chunks than its request's longest is cut in fewer parts
   const int32_t most = n > p.uncut ? (n + p.least - 1) / p.least : 1;
   t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
+  if (w.record + w.parts > p.limit) {
+    if (p.always) return false;
+    t.parts = 1;
+  }
   if (w.part >= t.parts) return false;
   const int32_t each = n / t.parts, more = n - each * t.parts;  // the first `more` parts have one chunk more
   t.t0 = each * w.part + (w.part < more ? w.part : more);
@@ -409,19 +427,23 @@ __device__ __forceinline__ void split_finite(u32x4_t& v, u32x4_t& up, u32x4_t& d
   }
 }
 
-// Zeros (lse -inf) for the tokens behind the last request, shared by all workgroups.
+// Zeros (lse -inf) for the tokens outside [head, live), the requests', shared by
+// all workgroups.
 template <int kThreads>
-__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t live, int32_t block, int32_t blocks) {
-  const int64_t units = static_cast<int64_t>(a.num_tokens - live) * a.heads * (a.head_dim / 8);
-  uint4* const out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
-                                              static_cast<int64_t>(live) * a.heads * a.head_dim);
+__device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t head, int32_t live, int32_t block,
+                                          int32_t blocks) {
+  const int64_t row = static_cast<int64_t>(a.heads) * (a.head_dim / 8);  // 16-byte pieces of a token
+  const int64_t gap = live - head;
+  uint4* const out = reinterpret_cast<uint4*>(a.out);
   const int64_t at = static_cast<int64_t>(block) * kThreads + threadIdx.x;
   const int64_t step = static_cast<int64_t>(blocks) * kThreads;
-  for (int64_t i = at; i < units; i += step) out[i] = uint4{0, 0, 0, 0};
+  for (int64_t i = at; i < (a.num_tokens - gap) * row; i += step) out[i < head * row ? i : i + gap * row] = uint4{0, 0, 0, 0};
   if (a.lse == nullptr) return;
-  const int32_t tail = a.num_tokens - live;
-  for (int64_t i = at; i < static_cast<int64_t>(tail) * a.heads; i += step)
-    a.lse[(i / tail) * a.num_tokens + live + i % tail] = -__builtin_inff();
+  const int64_t rest = a.num_tokens - gap;
+  for (int64_t i = at; i < rest * a.heads; i += step) {
+    const int64_t t = i % rest;
+    a.lse[(i / rest) * a.num_tokens + (t < head ? t : t + gap)] = -__builtin_inff();
+  }
 }
 
 // Record of (part of a tile, K/V head).
@@ -479,7 +501,8 @@ __device__ __forceinline__ void wide_tile(const PagedAttnArgs& a, const PagedPas
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
-  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end, block, blocks);
+  if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
+    fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -934,7 +957,8 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
-  if (w.end < a.num_tokens && a.fill_tail && !p.shared) fill_tail<kThreads>(a, w.end, block, blocks);
+  if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
+    fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
   if (w.request < 0 || !make_tile(a, p, w, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
@@ -1266,6 +1290,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
   constexpr int kAtOnce = 64 / kLanes;  // parts per load
   const int lane = threadIdx.x & 63;
   const int32_t group = a.heads / a.kv_heads;
+  const int64_t head = static_cast<int64_t>(first_token(a)) * group;
   const int64_t rows = static_cast<int64_t>(live_tokens(a)) * group;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
   const int32_t kvh = static_cast<int32_t>(id % a.kv_heads);
@@ -1277,7 +1302,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
     mo = own.meta[r0 + lane];
     if (pre.combined) mp = pre.meta[r0 + lane];
   }
-  uint64_t todo = __ballot(lane < n && (own.always || (mo.y & 0xffff) > 1));
+  const auto sound = [](const PagedPass& p, const int2& m) {
+    const int32_t parts = m.y & 0xffff;
+    return m.x >= 0 && m.x < p.limit && parts <= p.limit - m.x && (m.y >> 16) >= 0 && (m.y >> 16) < p.rows;
+  };
+  uint64_t todo = __ballot(lane < n && r0 + lane >= head && (own.always || (mo.y & 0xffff) > 1) && sound(own, mo) &&
+                           (!pre.combined || sound(pre, mp)));
   while (todo != 0) {
     const int i = __builtin_ctzll(todo);
     todo &= todo - 1;
@@ -1395,23 +1425,34 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
 }
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
-                 int32_t prefix_len, int64_t window, int64_t sinks, void* workspace, bool counters) {
+                 int32_t prefix_len, int64_t window, int64_t sinks, bool causal, void* workspace, bool counters) {
   Layout l{};
   const int64_t group = heads / kv_heads;
   const int64_t rows = tokens * group;
   const int64_t busy = requests < tokens ? requests : tokens;  // requests with queries
   const int64_t prefix_chunks = (static_cast<int64_t>(prefix_len) + kBN - 1) / kBN;
-  int64_t longest = (table_rows + kBN - 1) / kBN;  // chunks of a tile
-  const int64_t seen = (window + tokens) / kBN + 2 + (sinks + kBN - 1) / kBN;
-  if (window > 0 && seen < longest) longest = seen;
-  bool narrow = rows <= kNarrowRows * busy;
+  const int64_t table_chunks = (table_rows + kBN - 1) / kBN;
   // A prefix has a pass of its own where its rows are read by few rows per
-  // request; else it heads each tile's keys.
-  l.shared = prefix_len > 0 && rows < 64 * busy && !(narrow && busy * prefix_chunks * kv_heads <= 2048);
+  // request; else, and where it is short, it heads each tile's keys.
+  l.shared = prefix_len > 0 && rows < 64 * busy && busy * prefix_chunks * kv_heads > 2048;
+  // 16-row tiles up to 16 rows per request; up to 48 (up to three readings of its
+  // keys) where those are few or the prefix's tiles run beside them.
+  const bool light = busy * (table_chunks + prefix_chunks) * kv_heads <= 2048;
+  bool narrow = rows <= (l.shared || light ? 3 : 1) * kNarrowRows * busy;
+  const auto set_rows = [&](PagedPass& p, bool narrow) {
+    p.rows = narrow ? kNarrowRows : kWideRows;
+    p.tile_tokens = static_cast<int32_t>((p.rows + 2 * group - 2) / group);
+  };
+  set_rows(l.own, narrow);
+  int64_t longest = table_chunks;  // of a tile
+  if (window > 0) {
+    const int64_t span = causal && l.own.tile_tokens < tokens ? l.own.tile_tokens : tokens;
+    const int64_t seen = (window + span) / kBN + 2 + (sinks + kBN - 1) / kBN;
+    if (seen < longest) longest = seen;
+  }
   l.own.with_prefix = prefix_len > 0 && !l.shared;
   if (l.own.with_prefix) longest += prefix_chunks;
   l.own.always = l.shared;
-  l.own.rows = narrow ? kNarrowRows : kWideRows;
   const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
   l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
   l.own_units = units_bound(l.own, tiles, longest);
@@ -1424,9 +1465,10 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   // records: of tiles that are cut, at most twice the cuts; of all where all are joined
   auto place = [&](PagedPass& p, int64_t units, int64_t tiles) {
     char* const base = static_cast<char*>(workspace);
-    const int64_t cuts = units - tiles;
+    const int64_t limit = p.always ? units : 2 * (units - tiles) + 1;
+    p.limit = static_cast<int32_t>(limit < 0x7fffffff ? limit : 0x7fffffff);
     p.records = reinterpret_cast<float*>(base + at);
-    at += round256((p.always ? units : 2 * cuts + 1) * kv_heads * p.rows * (dim + 2) * 4);
+    at += round256(limit * kv_heads * p.rows * (dim + 2) * 4);
     p.meta = reinterpret_cast<int2*>(base + at);
     at += round256(rows * 8);
   };
@@ -1435,7 +1477,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     l.pre = l.own;
     l.pre.shared = 1;
     narrow = rows <= kNarrowRows;
-    l.pre.rows = narrow ? kNarrowRows : kWideRows;
+    set_rows(l.pre, narrow);
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
     l.pre_form = shape(l.pre, narrow, tiles, prefix_chunks, kv_heads);
     l.together = l.own_form != kWide;
@@ -1454,7 +1496,7 @@ template <int DT, int D>
 hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream) {
   const Layout l = layout_of(a.num_tokens, a.requests, a.heads, a.kv_heads, D,
                              static_cast<int64_t>(a.table_width) << a.block_shift, a.prefix_len, a.window, a.sinks,
-                             a.workspace, a.counters != nullptr);
+                             a.causal != 0, a.workspace, a.counters != nullptr);
   const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
@@ -1493,8 +1535,8 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
 }  // namespace
 
 int64_t paged_attention_workspace(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t head_dim,
-                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks) {
-  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, window, sinks, nullptr,
+                                  int64_t table_rows, int32_t prefix_len, int32_t window, int32_t sinks, bool causal) {
+  return layout_of(tokens, requests, heads, kv_heads, head_dim, table_rows, prefix_len, window, sinks, causal, nullptr,
                    false).bytes;
 }
 

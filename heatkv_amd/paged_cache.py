@@ -291,7 +291,7 @@ def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_ta
     lse = torch.empty((heads, T), dtype=torch.float32, device=device) if return_lse else None
     lib = _lib.load()
     need = int(lib.hkv_paged_attention_workspace_bytes(T, R, heads, kv_heads, dim, M, block, prefix_length,
-                                                       window, sinks))
+                                                       window, sinks, 1 if causal else 0))
     _lib.check(min(need, 0))
     ws = torch.empty((need,), dtype=torch.uint8, device=device) if need > 0 else None
     _call(device, lib.hkv_paged_attention, q.data_ptr(), int(q.stride(0)), int(q.stride(1)), k_cache.data_ptr(),

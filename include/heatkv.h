@@ -502,7 +502,8 @@ int32_t hkv_paged_append(const void* k, const void* v, int64_t k_token_stride, i
 int64_t hkv_paged_attention_counter_bytes(void);
 int64_t hkv_paged_attention_workspace_bytes(int32_t num_tokens, int32_t requests, int32_t heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t table_width, int32_t block_size,
-                                            int32_t prefix_length, int32_t window, int32_t sinks);
+                                            int32_t prefix_length, int32_t window, int32_t sinks,
+                                            int32_t causal);
 int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
                             const void* v_cache, int64_t k_block_stride, int64_t k_head_stride,
                             int64_t k_row_stride, int64_t v_block_stride, int64_t v_head_stride,
