@@ -842,6 +842,8 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
     return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes head_dim 64 or 128 (got %d)", head_dim);
   if (dtype != HKV_DTYPE_F16 && dtype != HKV_DTYPE_BF16)
     return fail(HKV_ERR_UNSUPPORTED, "the paged cache takes float16 or bfloat16 (got dtype code %d)", dtype);
+  if (!(softmax_scale - softmax_scale == 0.f))
+    return fail(HKV_ERR_INVALID_ARG, "softmax_scale must be finite");
   if ((static_cast<int64_t>(table_width) << shift) > 0x7fffff00LL || prefix_length > 0x7fffff00)
     return fail(HKV_ERR_UNSUPPORTED, "a table of more than 2^31 rows");
   if (static_cast<int64_t>(num_tokens) * (heads / kv_heads) > 0x7fffff00LL)

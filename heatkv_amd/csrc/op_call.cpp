@@ -425,6 +425,16 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
   return out;
 }
 
+// Elements [offset, offset + n) of a one-dimensional tensor, sharing its storage
+// (0.1 us where a dispatched view takes 1 and an allocation of its own 0.9).
+at::Tensor piece(const at::Tensor& base, int64_t offset, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()),
+                                                   c10::DispatchKeySet(c10::DispatchKey::CUDA), base.dtype());
+  impl->set_storage_offset(base.storage_offset() + offset);
+  impl->set_sizes_contiguous({n});
+  return at::Tensor(std::move(impl));
+}
+
 // paged_tables(block_tables, lengths, new_counts, free_blocks, free_range,
 // num_tokens, block_size, window, sinks, in_place): (slot_map, query_starts, lengths,
 // free_range, status)
@@ -448,10 +458,10 @@ PyObject* paged_tables_call(PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   const auto options = lengths.options();
   at::Tensor slots = at::empty({tokens}, options.dtype(at::kLong));
-  at::Tensor starts = at::empty({R + 1}, options);
-  at::Tensor status = at::empty({3}, options);
-  at::Tensor lengths_out = in_place ? lengths : at::empty({R}, options);
-  at::Tensor range_out = in_place ? range : at::empty({2}, options);
+  at::Tensor small = at::empty({2 * R + 6}, options);
+  at::Tensor starts = piece(small, 0, R + 1), status = piece(small, R + 1, 3);
+  at::Tensor range_out = in_place ? range : piece(small, R + 4, 2);
+  at::Tensor lengths_out = in_place ? lengths : piece(small, R + 6, R);
   int32_t code;
   Py_BEGIN_ALLOW_THREADS
   code = g.paged_tables(static_cast<int32_t*>(tables.data_ptr()), tables.stride(0), i32(lengths), i32(counts),
@@ -463,7 +473,7 @@ PyObject* paged_tables_call(PyObject* const* args, Py_ssize_t n) {
                         static_cast<int32_t*>(status.data_ptr()), stream);
   Py_END_ALLOW_THREADS
   if (code != HKV_OK) Py_RETURN_NONE;
-  at::Tensor first = status.narrow(0, 0, 1);
+  at::Tensor first = piece(small, R + 1, 1);
   if (!in_place) return tuple_of({slots, starts, lengths_out, range_out, first});
   Ref a(THPVariable_Wrap(slots)), b(THPVariable_Wrap(starts)), c(THPVariable_Wrap(first));
   if (a.p == nullptr || b.p == nullptr || c.p == nullptr) return nullptr;

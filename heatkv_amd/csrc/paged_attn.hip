@@ -53,7 +53,7 @@ struct PagedPass {
   int32_t combined;  // a combine launch follows: write meta
   int32_t join;      // the last part of a cut tile joins its records (counters)
   float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
-  int32_t limit;     // records there is room for (reached only by query_starts that are not ascending)
+  int32_t limit;     // records there is room for
   int2* meta;        // per live row: first record, parts | row in tile << 16
 };
 
@@ -305,12 +305,14 @@ struct Tile {
 };
 
 // Whether there is work; part and tile of `w` as its tile cuts them.
-__device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPass& p, const Work& w, Tile& t) {
+__device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPass& p, const Work& w, int32_t unit,
+                                          int32_t units, Tile& t) {
   const int32_t group = a.heads / a.kv_heads;
   t.g = w.g;
   t.row0 = w.tile * p.rows;
   t.rows = t.g.n * group - t.row0;
   t.rows = t.rows < p.rows ? t.rows : p.rows;
+  if (w.tile < 0 || t.rows <= 0) return false;
   const int32_t i0 = t.row0 / group, i1 = (t.row0 + t.rows - 1) / group;
   t.one = i0 == i1;
   t.keys = keys_of(a, p, t.g, i0, i1);
@@ -319,7 +321,9 @@ __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPas
   // a tile with fewer chunks than its request's longest is cut in fewer parts
   const int32_t most = n > p.uncut ? (n + p.least - 1) / p.least : 1;
   t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
-  if (w.record + w.parts > p.limit) {
+  // Where query_starts do not ascend, tiles may be more than the launch has room for:
+  // one without a record or a unit for each part is not cut.
+  if (w.record + w.parts > p.limit || unit - w.part + w.parts > units) {
     if (p.always) return false;
     t.parts = 1;
   }
@@ -369,7 +373,7 @@ __device__ __forceinline__ Sight sight_of(const PagedAttnArgs& a, const PagedPas
     const int32_t pos = g.len - g.n + i;
     if (pos < 0) s.hi = 0;
     else if (a.causal) s.hi = pos + 1;
-    if (a.window > 0) s.lo = pos - a.window + 1;
+    if (a.window > 0 && pos >= a.window) s.lo = pos - a.window + 1;
   }
   return s;
 }
@@ -504,7 +508,7 @@ __device__ __forceinline__ void wide_tile(const PagedAttnArgs& a, const PagedPas
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
-  if (w.request < 0 || !make_tile(a, p, w, t)) return;
+  if (w.request < 0 || !make_tile(a, p, w, unit, blocks / a.kv_heads, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
 
   // this lane's row (rows past the tile's last repeat it and are not stored)
@@ -960,7 +964,7 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
-  if (w.request < 0 || !make_tile(a, p, w, t)) return;
+  if (w.request < 0 || !make_tile(a, p, w, unit, blocks / a.kv_heads, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
 
   const int32_t mat = t.row0 + (q < t.rows ? q : t.rows - 1);

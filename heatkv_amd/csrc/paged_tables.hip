@@ -179,9 +179,9 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(const PagedTable
     const int32_t x = rows[r];
     return (x & kEnded) != 0 ? request_of(a, x & ~kEnded, -1) : request_of(a, x, starts[r + 1] - starts[r]);
   };
-  // Slot of each token: its request's block of the row, and the row in it.
-  for (int64_t t = at; t < a.num_tokens; t += step) {
-    int64_t slot = -1;
+  // Slot of a token: its request's block of the row, and the row in it.
+  const auto slot = [&](int64_t t) {
+    int64_t to = -1;
     if (fine && t < carry.tokens) {
       const int32_t r = find(starts, R, static_cast<uint32_t>(t));
       const int64_t row = (rows[r] & ~kEnded) + (t - starts[r]);
@@ -189,17 +189,15 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(const PagedTable
       const int64_t have = ((rows[r] & ~kEnded) + (1LL << a.block_shift) - 1) >> a.block_shift;
       const int64_t b = j < have ? a.block_tables[r * a.table_stride + j]
                                  : a.free_blocks[ring_at(popped[r] + (j - have))];
-      slot = (b << a.block_shift) + (row & ((1LL << a.block_shift) - 1));
+      to = (b << a.block_shift) + (row & ((1LL << a.block_shift) - 1));
     }
-    a.slot_map[t] = slot;
-  }
-  if (!fine) return;
-  for (int64_t i = at; i < carry.popped; i += step) {
+    a.slot_map[t] = to;
+  };
+  const auto pop = [&](int64_t i) {
     const int32_t r = find(popped, R, static_cast<uint32_t>(i));
     a.block_tables[r * a.table_stride + request(r).have + (i - popped[r])] = a.free_blocks[ring_at(i)];
-  }
-  if (alone) __syncthreads();
-  for (int64_t i = at; i < carry.pushed; i += step) {
+  };
+  const auto push = [&](int64_t i) {
     const int32_t r = find(pushed, R, static_cast<uint32_t>(i));
     const Request q = request(r);
     const int64_t k = i - pushed[r];
@@ -208,7 +206,21 @@ __global__ __launch_bounds__(kThreads) void paged_tables_kernel(const PagedTable
     const int32_t b = j < q.have || alone ? a.block_tables[r * a.table_stride + j]
                                           : a.free_blocks[ring_at(popped[r] + (j - q.have))];
     a.free_blocks[ring_at(static_cast<int64_t>(free) + i)] = b;
+  };
+  const int64_t tokens = a.num_tokens, pops = fine ? carry.popped : 0, pushes = fine ? carry.pushed : 0;
+  if (!alone) {
+    // side by side, so that no thread waits for one kind before it begins the next
+    for (int64_t i = at; i < tokens + pops + pushes; i += step) {
+      if (i < tokens) slot(i);
+      else if (i < tokens + pops) pop(i - tokens);
+      else push(i - tokens - pops);
+    }
+    return;
   }
+  for (int64_t i = at; i < tokens; i += step) slot(i);
+  for (int64_t i = at; i < pops; i += step) pop(i);
+  __syncthreads();
+  for (int64_t i = at; i < pushes; i += step) push(i);
 }
 
 // The state in place, once no workgroup of the step reads the old one any more.
@@ -264,9 +276,8 @@ typedef uint32_t U16B __attribute__((ext_vector_type(4)));
 }  // namespace
 
 hipError_t launch_paged_tables(const PagedTablesArgs& a, hipStream_t stream) {
-  // a workgroup per 1024 tokens, or per 32 requests whose blocks may move
-  int64_t blocks = (a.num_tokens + 1023LL) / 1024;
-  if (blocks < a.requests / 32) blocks = a.requests / 32;
+  // a workgroup per 1024 tokens, and per 32 requests whose blocks may move
+  int64_t blocks = (a.num_tokens + 1023LL) / 1024 + a.requests / 32;
   blocks = blocks < 1 ? 1 : (blocks > 128 ? 128 : blocks);
   const dim3 grid(static_cast<uint32_t>(blocks));
   if (a.requests <= 256 && blocks == 1) paged_tables_kernel<256><<<grid, 256, 0, stream>>>(a);

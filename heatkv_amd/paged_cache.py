@@ -20,6 +20,7 @@ The reference has no counterpart: its cache is one lockstep batch
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -259,6 +260,9 @@ def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_ta
     _check_ints("lengths", lengths, (R,), device)
     _check_ints("query_starts", query_starts, (R + 1,), device)
     window, sinks = _check_window(window, sinks)
+    softmax_scale = float(softmax_scale)
+    if not math.isfinite(softmax_scale):
+        raise ValueError(f"softmax_scale must be finite (got {softmax_scale})")
     prefix_length = int(prefix_length)
     if prefix_length < 0 or prefix_length >= 2**31:
         raise ValueError(f"prefix_length must lie in [0, 2^31) (got {prefix_length})")
@@ -299,7 +303,7 @@ def _attention(name, q, k_cache, v_cache, prefix_blocks, prefix_length, block_ta
           block_tables.data_ptr(), int(block_tables.stride(0)), lengths.data_ptr(), query_starts.data_ptr(),
           prefix_blocks.data_ptr() if prefix_length > 0 else None, prefix_length, out.data_ptr(),
           lse.data_ptr() if lse is not None else None, T, R, M, n, heads, kv_heads, dim, block, window, sinks,
-          1 if causal else 0, _lib.dtype_code(q.dtype), float(softmax_scale), 1 if fill else 0,
+          1 if causal else 0, _lib.dtype_code(q.dtype), softmax_scale, 1 if fill else 0,
           ws.data_ptr() if ws is not None else None, need,
           _lib.paged_counters(device).data_ptr() if need > 0 else None)
     return (out, lse) if return_lse else out
@@ -340,11 +344,16 @@ def paged_window_attention(
     query of the request sees are not read, nor their table entries.  Values
     that a query does not see (infinities and NaN included) have no effect on
     it.  A query that stands before row 0 sees nothing; such queries get zeros
-    (lse -inf).
+    (lse -inf).  Lengths beyond the table's rows count as those, and table
+    entries that name no block of the cache stand for block 0.
 
     Returns ``[T, H * D]`` in q's dtype and, with ``return_lse``, the fp32
-    log-sum-exp ``[H, T]``.  Tokens behind the last request get zeros (lse
-    -inf); with ``out`` (``[T, H * D]``, contiguous) they keep what it held.
+    log-sum-exp ``[H, T]``.  Tokens outside the requests' (before
+    ``query_starts[0]``, behind ``query_starts[R]``) get zeros (lse -inf); with
+    ``out`` (``[T, H * D]``, contiguous) they keep what it held.
+
+    Weights are rounded to q's 16-bit type for their product with V, as the
+    segmented attention's are; scores, maxima, sums and accumulators are fp32.
     """
     return _attention("paged_window_attention", q, k_cache, v_cache, None, 0, block_tables, lengths, query_starts,
                       softmax_scale, window, sinks, causal, out, return_lse)

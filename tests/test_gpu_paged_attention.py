@@ -202,3 +202,43 @@ def test_offsets_past_32_bits(device, counts):
     a["block_tables"] = torch.where((a["block_tables"] >= 0) & (a["block_tables"] < n),
                                     a["block_tables"] + (big - n), a["block_tables"])
     assert torch.equal(paged_window_attention(**a), want)
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 2], [60, 3, 40]])
+def test_the_widest_windows(device, counts):
+    """A window (and sinks) up to 2^31 - 1 is no window."""
+    b = Batch([300, 40, 90], counts, 4, 2)
+    want = paged_window_attention(**b.kwargs())
+    for window, sinks in ((2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (1, 2**31 - 1), (300, 0)):
+        assert torch.equal(paged_window_attention(**b.kwargs(), window=window, sinks=sinks), want)
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [50, 1, 130]])
+@pytest.mark.parametrize("prefix", [0, 2500])
+def test_a_part_of_a_batch(device, counts, prefix):
+    """Requests 1 and 2 of three: the tokens of request 0 are not theirs."""
+    b = Batch([5000, 700, 300], counts, 8, 2, prefix=prefix)
+    fn = paged_shared_prefix_attention if prefix else paged_window_attention
+    a = b.kwargs()
+    whole, lse = fn(**a, return_lse=True)
+    a.update(block_tables=a["block_tables"][1:], lengths=a["lengths"][1:], query_starts=a["query_starts"][1:])
+    n = counts[0]
+    out, l = fn(**a, return_lse=True)
+    b.check(out, l, slice(n, None))
+    assert (out[:n] == 0).all() and (l[:, :n] == -float("inf")).all()
+    mine = torch.full_like(out, 5.0)
+    fn(**a, out=mine)
+    assert (mine[:n] == 5).all() and torch.equal(mine[n:], out[n:])
+
+
+@pytest.mark.parametrize("prefix", [0, 2500])
+def test_query_starts_out_of_order(device, prefix):
+    """Starts that are not ascending (a caller's mistake) stay within every buffer:
+    what comes out is of no meaning, and the calls after it are as before."""
+    b = Batch([5000, 700, 300], [40, 2, 90], 8, 2, prefix=prefix)
+    fn = paged_shared_prefix_attention if prefix else paged_window_attention
+    a = b.kwargs()
+    want = fn(**a)
+    for starts in ([0, 132, 0, 132], [132, 0, 132, 0], [-5, 9000, 7, -1]):
+        fn(**{**a, "query_starts": torch.tensor(starts, dtype=torch.int32, device=device)})
+    assert torch.equal(fn(**a), want)

@@ -91,6 +91,8 @@ def test_cache_refusals():
     (dict(query_starts=i32(3)), ValueError, "query_starts"),
     (dict(lengths=i32(2)), ValueError, "lengths"),
     (dict(window=-5), ValueError, "window"),
+    (dict(softmax_scale=float("nan")), ValueError, "finite"),
+    (dict(softmax_scale=float("inf")), ValueError, "finite"),
     (dict(out=torch.zeros((5, 512))), ValueError, "out must be"),
     (dict(out=torch.zeros((5, 1024), dtype=torch.bfloat16)[:, ::2]), ValueError, "contiguous"),
     (dict(), RuntimeError, "requires CUDA tensors"),
@@ -127,11 +129,11 @@ def test_abi_refusals_before_any_device_call():
     assert append(4, 1, 2, 128, 16) == _lib.HKV_ERR_INVALID_ARG
     assert append(4, 0, 2, 128, 16) == 0
 
-    def attn(T=1, R=1, M=4, N=4, H=4, hk=2, D=128, block=16, dtype=2, strides=128, prefix=0):
+    def attn(T=1, R=1, M=4, N=4, H=4, hk=2, D=128, block=16, dtype=2, strides=128, prefix=0, scale=1.0):
         import ctypes
         return lib.hkv_paged_attention(n, strides, strides, n, n, strides, strides, strides, strides, strides, strides,
                                        n, M, n, n, n, prefix, n, n, T, R, M, N, H, hk, D, block, 0, 0, 1, dtype,
-                                       ctypes.c_float(1.0), 1, n, 0, n, n)
+                                       ctypes.c_float(scale), 1, n, 0, n, n)
     assert attn(H=3) == _lib.HKV_ERR_INVALID_ARG
     assert attn(D=96) == _lib.HKV_ERR_UNSUPPORTED
     assert attn(dtype=3) == _lib.HKV_ERR_UNSUPPORTED
@@ -140,6 +142,7 @@ def test_abi_refusals_before_any_device_call():
     assert attn(R=5000) == _lib.HKV_ERR_UNSUPPORTED
     assert attn(T=2**30, H=8, hk=1) == _lib.HKV_ERR_UNSUPPORTED
     assert attn() == _lib.HKV_ERR_INVALID_ARG
+    assert attn(scale=float("nan")) == _lib.HKV_ERR_INVALID_ARG and "finite" in _lib.last_error()
     assert attn(T=0) == 0
 
 
