@@ -5,19 +5,28 @@
 // The queries of one request and K/V head are a matrix of n * group rows (token
 // by token, the heads of a group side by side) against one stream of keys.  Two
 // kernels run tiles of those rows:
-//  * paged_wide_kernel, 128 rows, matrix-bound: prompts and scales.
-//  * paged_narrow_kernel, 16 rows, bound by the bytes of the cache: single tokens.
+//  * wide_tile, 128 rows: prompts and scales, bound by the matrix cores (and, as
+//    the segmented kernel, by the chains of its softmax).  A prompt of 8192 tokens,
+//    32 heads on 8: 560 us, 980 TFLOP/s; library products of random bf16 reach
+//    1130 to 1350 on the same card.
+//  * narrow_tile, 16 rows: single tokens, bound by the bytes of the cache.  64
+//    requests of 800 to 16000 rows, 2.33 GB: 404 us, 5.8 TB/s; a copy of 2 GiB
+//    moves 4.95.
 //
 // Plan.  Nothing about the requests is known on the host, so every workgroup
-// finds its work from lengths and query_starts itself: tiles of rows per
+// finds its work from lengths and query_starts itself (1 to 2 us, beside other
+// workgroups' work in all but the smallest launches; a plan made by a launch of its
+// own would cost every call that much): tiles of rows per
 // request, 64-key chunks per tile, and, so that few rows over long keys still
-// fill the card, `parts` of a tile's chunks.  With `total` chunks in the launch
-// a part has c = max(least, total / units wanted) of them, so there are at most
-// tiles + wanted units per K/V head (the grid) and 2 * wanted of them belong
-// to tiles that are cut (their partial results' records).  A tile that is not
-// cut writes its output; the parts of the others leave an unnormalized O, a
-// maximum and a sum, which paged_combine_kernel joins in part order, so results do
-// not depend on the order of arrival and nothing has to be cleared or waited for.
+// fill the card, parts of a tile's chunks.  part_chunks gives the chunks of a
+// part from the total of the launch, so that the host knows how many units and
+// records there can be at most.  A tile that is not cut writes its output.  Parts of
+// narrow tiles are joined by the last of them (join_parts): a pair of tokens over
+// 6425 rows, 16 heads, 27.3 us against 30.7 with a launch for it.  Parts of wide
+// tiles, whose records are 66 KB, and the prefix's and own results of one row are
+// joined by paged_combine_kernel (joining wide parts in place: 8 requests of 17
+// tokens behind 1000 rows 50 us against 22).  Either way in part order, so results do
+// not depend on the order of arrival.
 #include "attn_common.h"
 #include "paged.h"
 
@@ -39,33 +48,34 @@ constexpr float kNoMax = -1e30f;
 // One launch: the requests' own rows, or (shared) the prefix for the rows of
 // all requests together.
 struct PagedPass {
-  int32_t shared;    // one pseudo request: all live tokens, the prefix's keys
-  int32_t with_prefix;  // each tile's keys begin with the prefix (wide tiles that need no sharing)
-  int32_t rows;      // rows of a tile
+  int32_t shared;       // one pseudo request: all live tokens, the prefix's keys
+  int32_t with_prefix;  // each tile's keys begin with the prefix
+  int32_t rows;         // rows of a tile
   int32_t tile_tokens;  // tokens that a tile spans at most
-  int32_t least;     // chunks of a part at least
-  int32_t wanted;    // units per K/V head that fill the card once
-  int32_t most;      // ... and that parts may make at most
-  int32_t cap;       // chunks of a part from which more than `wanted` are made
-  int32_t step;      // parts are multiples of this many chunks
-  int32_t uncut;     // tiles of up to this many chunks are not cut
-  int32_t always;    // every tile leaves records (a shared prefix is joined to it)
-  int32_t combined;  // a combine launch follows: write meta
-  int32_t join;      // the last part of a cut tile joins its records (counters)
-  float* records;    // per record and K/V head: rows * D values, rows maxima, rows sums
-  int32_t limit;     // records there is room for
-  int2* meta;        // per live row: first record, parts | row in tile << 16
+  int32_t least;        // chunks of a part at least
+  int32_t wanted;       // units per K/V head that fill the card once
+  int32_t most;         // ... and that parts may make at most
+  int32_t cap;          // chunks of a part from which more than `wanted` are made
+  int32_t step;         // parts are multiples of this many chunks (a power of two)
+  int32_t uncut;        // tiles of up to this many chunks are not cut
+  int32_t always;       // every tile leaves records (a shared prefix's are joined to them)
+  int32_t combined;     // a combine launch follows: write meta
+  int32_t join;         // the last part of a cut tile joins its records (counters)
+  int32_t limit;        // records there is room for
+  float* records;       // per record and K/V head: rows * D values, rows maxima, rows sums
+  int2* meta;           // per live row: first record, parts | row in tile << 16
 };
 
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Chunks of a part in a launch of `total` chunks (per K/V head): total / c, the
-// number of parts, never falls with total and is at most `most`.
 __host__ __device__ __forceinline__ int64_t up_div(int64_t a, int32_t b) {
   // 32-bit where that does (64-bit divisions cost about 150 instructions)
   const int64_t n = a + b - 1;
   return n >> 32 == 0 ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(b)) : n / b;
 }
+
+// Chunks of a part in a launch of `total` chunks (per K/V head): enough units to fill
+// the card once, more where parts would be longer than `cap`.
 __host__ __device__ __forceinline__ int64_t part_chunks(const PagedPass& p, int64_t total) {
   int64_t c = up_div(total, p.wanted);
   if (c > p.cap) {
@@ -441,7 +451,8 @@ __device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t head, 
   uint4* const out = reinterpret_cast<uint4*>(a.out);
   const int64_t at = static_cast<int64_t>(block) * kThreads + threadIdx.x;
   const int64_t step = static_cast<int64_t>(blocks) * kThreads;
-  for (int64_t i = at; i < (a.num_tokens - gap) * row; i += step) out[i < head * row ? i : i + gap * row] = uint4{0, 0, 0, 0};
+  for (int64_t i = at; i < (a.num_tokens - gap) * row; i += step)
+    out[i < head * row ? i : i + gap * row] = uint4{0, 0, 0, 0};
   if (a.lse == nullptr) return;
   const int64_t rest = a.num_tokens - gap;
   for (int64_t i = at; i < rest * a.heads; i += step) {
@@ -473,7 +484,9 @@ __device__ __forceinline__ void write_meta(const PagedAttnArgs& a, const PagedPa
 // one shares): chunks go straight to LDS, two stages, K one chunk ahead of V, so
 // iteration t runs S(t + 1) on the matrix cores beside the exponentials of S(t).
 // Waves 0 and 1 load the K rows, 2 and 3 the V rows, each lane the rows of its
-// own; the table entries of the next chunk are read one iteration ahead.
+// own (its address is made once per lane and chunk, V lanes take theirs from LDS:
+// 560 against 598 us a prompt of 8192 with an address for each of a V lane's four
+// rows); the table entries of the next chunk are read one iteration ahead.
 template <int D>
 struct WideLds {
   static constexpr int kTensor = kBN * D * 2;  // bytes of a chunk's K or V
@@ -804,15 +817,16 @@ __global__ __launch_bounds__(256, 2) void paged_wide_kernel(const PagedAttnArgs 
 
 // ---------------------------------------------------------------- narrow tiles
 //
-// 16 rows on the 16x16x32 MFMAs; bound by the bytes of the cache.  Two waves, each
-// with its own half (32 keys) of every chunk, its own stages in LDS and its own
-// softmax, joined at the end: no barrier in the loop.  Per stage a wave sends 32
+// 16 rows on the 16x16x32 MFMAs; bound by the bytes of the cache.  The 32-key
+// halves of the part's chunks are dealt to NW waves, each with its own stages in
+// LDS and its own softmax, joined at the end: no barrier in the loop.  Per stage a wave sends 32
 // rows of K and of V straight to LDS, whole rows side by side (16-byte pieces of
 // a row exchanged by its number, so that reads of one piece from 16 rows meet
-// 16 different banks).  Row addresses come from table entries that arrive in LDS the same way,
-// NS stages ahead of the rows, so no load is waited for but by count: a group is
-// the rows of stage k and the entries of stage k + NS, and NS - 1 younger groups
-// stay in flight.
+// 16 different banks).  Row addresses come from table entries that arrive in LDS
+// the same way, NS stages ahead of the rows, so no load is waited for but by
+// count: a group is the rows of stage k and the entries of stage k + NS, and NS - 1
+// younger groups stay in flight.  128 KB of the cache are in flight per CU either
+// way: two workgroups of two waves with two stages, or one of eight waves with one.
 template <int DT>
 __device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
   if constexpr (DT == kF16)
@@ -986,7 +1000,8 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   auto look_up = [&](int32_t k) {
     bool prefix;
     const int32_t j = stage_row(k, prefix) + (lane & 31);
-    dma4((prefix ? a.prefix_blocks : t.blocks) + (row_to_load(a, t.keys, j, prefix) >> a.block_shift), lds_address(my.ids[k % NS]));
+    dma4((prefix ? a.prefix_blocks : t.blocks) + (row_to_load(a, t.keys, j, prefix) >> a.block_shift),
+         lds_address(my.ids[k % NS]));
   };
   const bool for_k = lane < 32;
   PagedCacheStrides cs;
@@ -1245,7 +1260,9 @@ __global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAtt
 // The prefix's tiles (wide: bound by the matrix cores) and the requests' own (narrow:
 // bound by bytes) in one launch, so that each CU runs one of either.  Workgroups go
 // to the 8 XCDs in turn and to an XCD's 32 CUs in turn, twice: the kinds alternate
-// from CU to CU, and the other way round for a CU's second workgroup.
+// from CU to CU, and the other way round for a CU's second workgroup.  128 tokens
+// behind 16384 rows, 32 heads on 8: 88.9 us with the combine, 104.2 in two launches (51
+// and 43, and 11); 16 tokens behind 2000 rows, 16 heads: 18.8 / 25.2.
 template <int DT, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a, const PagedPass pre,
                                                               const PagedPass own, const Scalars sc,
@@ -1398,6 +1415,20 @@ int64_t units_bound(const PagedPass& p, int64_t tiles, int64_t chunks) {
 }
 
 // How a launch of up to `tiles` tiles (per K/V head) of up to `chunks` chunks runs.
+// 256 stands for the CUs.  us on the device:
+// * wide, few tiles: parts of 4 chunks and more, one unit per CU first (32 tiles of
+//   65 chunks: 32.1, two per CU 37.8) and two from 12 chunks a part (128 tiles of 135: 98
+//   against 110); up to 16 chunks whole (40 tiles of 15: 21 against 31).  Many tiles: up
+//   to 32 chunks whole (470 tiles of up to 14: 36 against 54; but 64 tiles of 33, 38
+//   cut, 65 whole).
+// * narrow, up to one tile and 32 chunks per CU: eight waves on one tile, whole up to 16
+//   chunks (8 heads, 300 rows 7.8, cut 10.3; 16 requests of 500 behind a prefix 10.3 / 13.9;
+//   1000 rows 11.4 / 10.7), else in parts of 4 and its multiples, a stage for each wave (8
+//   requests of up to 2000 rows: 14.0, in parts of 5 chunks 20.3, two waves on a tile 17.7).
+// * long tiles: eight waves, in parts of up to 48 chunks (64 requests of up to 16000 rows
+//   418, two waves 436; one of 64000 58 / 68); many short ones: two waves, two workgroups
+//   per CU (256 requests of up to 1200 rows 143, eight waves 160 to 169), whole up to 16
+//   chunks (32 requests of 1000 rows 30.7 / 34.7).
 Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_heads) {
   p.cap = 0x7fffffff;
   p.step = 1;
@@ -1437,10 +1468,14 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   const int64_t prefix_chunks = (static_cast<int64_t>(prefix_len) + kBN - 1) / kBN;
   const int64_t table_chunks = (table_rows + kBN - 1) / kBN;
   // A prefix has a pass of its own where its rows are read by few rows per
-  // request; else, and where it is short, it heads each tile's keys.
+  // request; else, and where it is short, it heads each tile's keys.  us, a pass of
+  // its own / heading the keys, by requests x chunks x K/V heads: 1760 14.4 / 9.7, 3608
+  // 14.6 / 16.1, 4096 20.9 / 18.9, 8192 18.8 / 32.
   l.shared = prefix_len > 0 && rows < 64 * busy && busy * prefix_chunks * kv_heads > 2048;
   // 16-row tiles up to 16 rows per request; up to 48 (up to three readings of its
-  // keys) where those are few or the prefix's tiles run beside them.
+  // keys) where those are few or the prefix's tiles run beside them.  us, 16-row /
+  // 128-row tiles: 32 requests over 2000 rows, 20 rows each 66.8 / 63.3, 36 rows 87 / 62; 36
+  // rows each behind 4000 rows 33.6 / 43; 18 rows each over 200 rows 8.6 / 12.9.
   const bool light = busy * (table_chunks + prefix_chunks) * kv_heads <= 2048;
   bool narrow = rows <= (l.shared || light ? 3 : 1) * kNarrowRows * busy;
   const auto set_rows = [&](PagedPass& p, bool narrow) {
@@ -1485,7 +1520,8 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     const int64_t tiles = (rows + l.pre.rows - 1) / l.pre.rows;
     l.pre_form = shape(l.pre, narrow, tiles, prefix_chunks, kv_heads);
     l.together = l.own_form != kWide;
-    if (l.together && l.pre_form == kWide) {  // one per CU beside the requests' own tiles
+    if (l.together && l.pre_form == kWide) {
+      // one per CU beside the requests' own tiles (two: 100 against 88.9 us above)
       l.pre.wanted = l.pre.most = (256 + kv_heads - 1) / kv_heads;
       l.pre.cap = 0x7fffffff;
     }

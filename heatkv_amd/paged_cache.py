@@ -149,8 +149,9 @@ def build_paged_tables(
     with ``in_place`` the given ones, updated) and ``status`` int32 ``[1]``: 0,
     or a sum of 1 (too few free blocks), 2 (a request does not fit its table
     row) and 4 (more tokens than ``num_tokens``), or 8 (more blocks given back
-    than the ring has room for).  A step with a nonzero status changes nothing: every slot is -1, every query start 0, and the state is
-    as before.  Calling it again with the same inputs gives the same results
+    than the ring has room for).  A step with a nonzero status changes nothing:
+    every slot is -1, every query start 0, and the state is as before.
+    Calling it again with the same inputs gives the same results
     (unless ``in_place``).
     """
     native = _lib.op_call
