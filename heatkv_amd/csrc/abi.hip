@@ -879,9 +879,9 @@ int32_t hkv_paged_attention(const void* q, int64_t q_token_stride, int64_t q_hea
   hkv::PagedAttnArgs a{q, q_token_stride, q_head_stride, k_cache, v_cache,
                        {k_block_stride, k_head_stride, k_row_stride}, {v_block_stride, v_head_stride, v_row_stride},
                        block_tables, table_stride, lengths, query_starts, prefix_blocks, prefix_length, out, lse,
-                       num_tokens, requests, table_width, num_blocks, heads, kv_heads, head_dim, shift, window, sinks,
-                       causal != 0 ? 1 : 0, dtype, fill_tail != 0 ? 1 : 0, softmax_scale, workspace, workspace_bytes,
-                       static_cast<int32_t*>(counters)};
+                       num_tokens, requests, table_width, num_blocks, heads, kv_heads, heads / kv_heads, head_dim, shift,
+                       window, sinks, causal != 0 ? 1 : 0, dtype, fill_tail != 0 ? 1 : 0, softmax_scale, workspace,
+                       workspace_bytes, static_cast<int32_t*>(counters)};
   const hipError_t e = hkv::launch_paged_attention(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(HKV_ERR_LAUNCH, "paged attention launch failed: %s", hipGetErrorString(e));
   return ok();

@@ -74,6 +74,7 @@ struct PagedAttnArgs {
   int32_t num_blocks;
   int32_t heads;
   int32_t kv_heads;
+  int32_t group;  // heads / kv_heads
   int32_t head_dim;
   int32_t block_shift;
   int32_t window;  // 0: none

@@ -62,6 +62,7 @@ struct PagedPass {
   int32_t combined;     // a combine launch follows: write meta
   int32_t join;         // the last part of a cut tile joins its records (counters)
   int32_t limit;        // records there is room for
+  int32_t units;        // units there are workgroups for (per K/V head)
   float* records;       // per record and K/V head: rows * D values, rows maxima, rows sums
   int2* meta;           // per live row: first record, parts | row in tile << 16
 };
@@ -156,7 +157,7 @@ struct Load {
 };
 
 __device__ __forceinline__ Load load_of(const PagedAttnArgs& a, const PagedPass& p, const Geometry& g) {
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   Load l{0, 0};
   if (g.n == 0) return l;
   l.tiles = (g.n * group + p.rows - 1) >> (p.rows == kWideRows ? 7 : 4);
@@ -213,14 +214,18 @@ template <int kThreads>
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
-  Work w{-1, 0, 0, 1, 0, {0, 0, 0}, first_token(a), live_tokens(a)};
-  if (w.end < w.head) w.end = w.head;
+  Work w{-1, 0, 0, 1, 0, {0, 0, 0}, 0, 0};
   if (R <= 64) {
     Load l{0, 0};
     Geometry g{0, 0, 0};
     if (lane < R) {
       g = load_request(a, p, lane);
       l = load_of(a, p, g);
+    }
+    if (R > 0) {
+      w.head = __builtin_amdgcn_readlane(g.first, 0);
+      w.end = __builtin_amdgcn_readlane(g.first + g.n, R - 1);
+      if (w.end < w.head) w.end = w.head;
     }
     const int64_t total = wave_sum64(static_cast<int64_t>(l.tiles) * l.chunks, R);
     const int64_t c = part_chunks(p, total);
@@ -240,6 +245,9 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
                    __builtin_amdgcn_readlane(g.len, src)};
     return w;
   }
+  w.head = first_token(a);
+  w.end = live_tokens(a);
+  if (w.end < w.head) w.end = w.head;
   constexpr int kWaves = kThreads / 64;
   __shared__ int64_t wave_total[kWaves];
   __shared__ int2 wave_units[kWaves];
@@ -316,8 +324,8 @@ struct Tile {
 
 // Whether there is work; part and tile of `w` as its tile cuts them.
 __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPass& p, const Work& w, int32_t unit,
-                                          int32_t units, Tile& t) {
-  const int32_t group = a.heads / a.kv_heads;
+                                          Tile& t) {
+  const int32_t group = a.group;
   t.g = w.g;
   t.row0 = w.tile * p.rows;
   t.rows = t.g.n * group - t.row0;
@@ -333,7 +341,7 @@ __device__ __forceinline__ bool make_tile(const PagedAttnArgs& a, const PagedPas
   t.parts = w.parts < most ? w.parts : (most > 1 ? most : 1);
   // Where query_starts do not ascend, tiles may be more than the launch has room for:
   // one without a record or a unit for each part is not cut.
-  if (w.record + w.parts > p.limit || unit - w.part + w.parts > units) {
+  if (w.record + w.parts > p.limit || unit - w.part + w.parts > p.units) {
     if (p.always) return false;
     t.parts = 1;
   }
@@ -471,7 +479,7 @@ template <int kThreads>
 __device__ __forceinline__ void write_meta(const PagedAttnArgs& a, const PagedPass& p, const Tile& t, const Work& w,
                                            int32_t kvh) {
   if (!p.combined || w.part != 0 || kvh != 0) return;
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   for (int32_t i = threadIdx.x; i < t.rows; i += kThreads)
     p.meta[static_cast<int64_t>(t.g.first) * group + t.row0 + i] = int2{w.record, t.parts | i << 16};
 }
@@ -514,14 +522,14 @@ __device__ __forceinline__ void wide_tile(const PagedAttnArgs& a, const PagedPas
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5;
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
-  if (w.request < 0 || !make_tile(a, p, w, unit, blocks / a.kv_heads, t)) return;
+  if (w.request < 0 || !make_tile(a, p, w, unit, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
 
   // this lane's row (rows past the tile's last repeat it and are not stored)
@@ -883,7 +891,7 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const PagedPa
   const int wave = uniform(threadIdx.x >> 6);
   constexpr int kLanes = D / 2;         // of a part's row
   constexpr int kAtOnce = 64 / kLanes;  // parts per load
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * (p.rows * (D + 2));
   const float* const rec0 = record_of<D>(a, p, w.record, kvh);
   for (int32_t row = wave; row < t.rows; row += NW) {
@@ -971,14 +979,14 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   const int wave = uniform(tid >> 6);
   const int q = lane & 15;
   const int g = lane >> 4;
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
   const Work w = find_work<kThreads>(a, p, unit);
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
-  if (w.request < 0 || !make_tile(a, p, w, unit, blocks / a.kv_heads, t)) return;
+  if (w.request < 0 || !make_tile(a, p, w, unit, t)) return;
   write_meta<kThreads>(a, p, t, w, kvh);
 
   const int32_t mat = t.row0 + (q < t.rows ? q : t.rows - 1);
@@ -1310,7 +1318,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
   constexpr int kLanes = D / 4;         // of a part's row
   constexpr int kAtOnce = 64 / kLanes;  // parts per load
   const int lane = threadIdx.x & 63;
-  const int32_t group = a.heads / a.kv_heads;
+  const int32_t group = a.group;
   const int64_t head = static_cast<int64_t>(first_token(a)) * group;
   const int64_t rows = static_cast<int64_t>(live_tokens(a)) * group;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + uniform(threadIdx.x >> 6);
@@ -1495,6 +1503,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
   l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
   l.own_units = units_bound(l.own, tiles, longest);
+  l.own.units = static_cast<int32_t>(l.own_units < 0x7fffffff ? l.own_units : 0x7fffffff);
   const bool may_cut = longest > l.own.least && longest > l.own.uncut;
   // a record's counter is 8 bytes of the counters
   l.own.join = counters && may_cut && l.own_form != kWide && !l.shared &&
@@ -1526,6 +1535,7 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
       l.pre.cap = 0x7fffffff;
     }
     l.pre_units = units_bound(l.pre, tiles, prefix_chunks);
+    l.pre.units = static_cast<int32_t>(l.pre_units < 0x7fffffff ? l.pre_units : 0x7fffffff);
     place(l.pre, l.pre_units, tiles);
   }
   l.bytes = at;
@@ -1561,7 +1571,7 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !l.own.combined) return e;
-  const int64_t rows = static_cast<int64_t>(a.num_tokens) * (a.heads / a.kv_heads);
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * a.group;
   // about 8192 waves; where every row is joined, one each
   const int64_t per = l.own.always ? 1 : rows * a.kv_heads / 8192;
   const int32_t chunk = static_cast<int32_t>(per < 1 ? 1 : (per > 64 ? 64 : per));
