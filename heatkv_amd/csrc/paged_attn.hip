@@ -41,6 +41,7 @@ typedef __attribute__((address_space(3))) void* lds_void_ptr;
 
 constexpr int kWideRows = 128;
 constexpr int kNarrowRows = 16;
+constexpr int kPlanned = 64;  // requests that each wave plans by itself
 constexpr float kNoMax = -1e30f;
 
 // ---------------------------------------------------------------- plan
@@ -63,6 +64,7 @@ struct PagedPass {
   int32_t join;         // the last part of a cut tile joins its records (counters)
   int32_t limit;        // records there is room for
   int32_t units;        // units there are workgroups for (per K/V head)
+  const int4* list;     // the units' work, for more than kPlanned requests
   float* records;       // per record and K/V head: rows * D values, rows maxima, rows sums
   int2* meta;           // per live row: first record, parts | row in tile << 16
 };
@@ -199,23 +201,29 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t v, int n = 64) {
                               static_cast<uint64_t>(uniform(static_cast<int32_t>(v >> 32))) << 32);
 }
 
+// Counts of units and records that more than can be launched do not overflow.
+__device__ __forceinline__ int2 add_units(const int2& a, const int2& b) {
+  constexpr int32_t kMost = 0x3fffffff;
+  const int32_t x = a.x + b.x, y = a.y + b.y;
+  return int2{x < kMost ? x : kMost, y < kMost ? y : kMost};
+}
+
 __device__ __forceinline__ int2 wave_prefix(int2 v, int n = 64) {
   const int lane = threadIdx.x & 63;
   for (int off = 1; off < n; off <<= 1) {
     const int2 o{__shfl_up(v.x, off, 64), __shfl_up(v.y, off, 64)};
-    if (lane >= off) v = int2{v.x + o.x, v.y + o.y};
+    if (lane >= off) v = add_units(v, o);
   }
   return v;
 }
 
 // Work of unit `unit` (per K/V head).  Up to 64 requests every wave plans by
 // itself, a request per lane; more are dealt to the workgroup's threads in runs.
-template <int kThreads>
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
   Work w{-1, 0, 0, 1, 0, {0, 0, 0}, 0, 0};
-  if (R <= 64) {
+  if (R <= kPlanned) {
     Load l{0, 0};
     Geometry g{0, 0, 0};
     if (lane < R) {
@@ -245,69 +253,91 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
                    __builtin_amdgcn_readlane(g.len, src)};
     return w;
   }
-  w.head = first_token(a);
-  w.end = live_tokens(a);
-  if (w.end < w.head) w.end = w.head;
-  constexpr int kWaves = kThreads / 64;
+  // what paged_plan_kernel wrote
+  const int4 x = p.list[2 * static_cast<int64_t>(unit)], y = p.list[2 * static_cast<int64_t>(unit) + 1];
+  const int4 range = p.list[2 * static_cast<int64_t>(p.units)];
+  w.head = uniform(range.x);
+  w.end = uniform(range.y);
+  w.request = uniform(x.x);
+  w.tile = uniform(x.y);
+  w.part = uniform(x.z);
+  w.parts = uniform(x.w);
+  w.record = uniform(y.x);
+  w.g = Geometry{uniform(y.y), uniform(y.z), uniform(y.w)};
+  return w;
+}
+
+// The work of every unit of a launch of more than kPlanned requests, 32 bytes each, and
+// behind them the range of live tokens.  Each workgroup plans all requests, four to a
+// thread, and finds its own units' requests by bisection.
+__global__ __launch_bounds__(1024) void paged_plan_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                          int4* __restrict__ list) {
+  constexpr int kThreads = 1024, kWaves = kThreads / 64, kRun = kMaxRequests / kThreads;
   __shared__ int64_t wave_total[kWaves];
   __shared__ int2 wave_units[kWaves];
-  __shared__ int32_t found[8];
+  __shared__ int32_t start[kMaxRequests], record[kMaxRequests], tiles[kMaxRequests], cut[kMaxRequests];
   const int tid = threadIdx.x;
+  const int lane = tid & 63;
   const int wave = tid >> 6;
+  const int32_t R = a.requests;
   const int32_t run = (R + kThreads - 1) / kThreads;
-  const int32_t r0 = tid * run < R ? tid * run : R, r1 = r0 + run < R ? r0 + run : R;
+  const int32_t r0 = tid * run;
+  Load l[kRun];
   int64_t sum = 0;
-  for (int32_t r = r0; r < r1; ++r) {
-    const Load l = load_of(a, p, load_request(a, p, r));
-    sum += static_cast<int64_t>(l.tiles) * l.chunks;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    l[i] = Load{0, 0};
+    if (i < run && r0 + i < R) l[i] = load_of(a, p, load_request(a, p, r0 + i));
+    sum += static_cast<int64_t>(l[i].tiles) * l[i].chunks;
   }
   sum = wave_sum64(sum);
   if (lane == 0) wave_total[wave] = sum;
-  if (tid == 0) found[0] = -1;
   __syncthreads();
   int64_t total = 0;
   for (int i = 0; i < kWaves; ++i) total += wave_total[i];
   const int64_t c = part_chunks(p, total);
   int2 mine{0, 0};
-  for (int32_t r = r0; r < r1; ++r) {
-    const int2 u = units_of(p, load_of(a, p, load_request(a, p, r)), c);
-    mine = int2{mine.x + u.x, mine.y + u.y};
-  }
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) mine = add_units(mine, units_of(p, l[i], c));
   int2 end = wave_prefix(mine);
   if (lane == 63) wave_units[wave] = end;
+  int2 at{__shfl_up(end.x, 1, 64), __shfl_up(end.y, 1, 64)};
+  if (lane == 0) at = int2{0, 0};
   __syncthreads();
-  for (int i = 0; i < wave; ++i) end = int2{end.x + wave_units[i].x, end.y + wave_units[i].y};
-  int2 at{end.x - mine.x, end.y - mine.y};
-  if (unit >= at.x && unit < end.x) {  // one thread
-    for (int32_t r = r0; r < r1; ++r) {
-      const Geometry g = load_request(a, p, r);
-      const Load l = load_of(a, p, g);
-      const int2 u = units_of(p, l, c);
-      if (unit < at.x + u.x) {
-        const int32_t parts = parts_of(p, l, c);
-        const int32_t in = unit - at.x;
-        found[0] = r;
-        found[1] = l.tiles - 1 - in / parts;
-        found[2] = in % parts;
-        found[3] = parts;
-        found[4] = at.y + found[1] * parts;
-        found[5] = g.n;
-        found[6] = g.first;
-        found[7] = g.len;
-        break;
-      }
-      at = int2{at.x + u.x, at.y + u.y};
-    }
+  int2 all{0, 0};
+  for (int i = 0; i < kWaves; ++i) {
+    if (i == wave) at = add_units(all, at);
+    all = add_units(all, wave_units[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    if (i >= run || r0 + i >= R) break;
+    start[r0 + i] = at.x;
+    record[r0 + i] = at.y;
+    tiles[r0 + i] = l[i].tiles;
+    cut[r0 + i] = parts_of(p, l[i], c);
+    at = add_units(at, units_of(p, l[i], c));
   }
   __syncthreads();
-  w.request = __builtin_amdgcn_readfirstlane(found[0]);
-  if (w.request < 0) return w;
-  w.tile = __builtin_amdgcn_readfirstlane(found[1]);
-  w.part = __builtin_amdgcn_readfirstlane(found[2]);
-  w.parts = __builtin_amdgcn_readfirstlane(found[3]);
-  w.record = __builtin_amdgcn_readfirstlane(found[4]);
-  w.g = Geometry{uniform(found[5]), uniform(found[6]), uniform(found[7])};
-  return w;
+  for (int32_t u = blockIdx.x * kThreads + tid; u < p.units; u += gridDim.x * kThreads) {
+    int4 x{-1, 0, 0, 1}, y{0, 0, 0, 0};
+    if (u < all.x) {
+      int32_t r = 0;  // the last request that starts at or before u
+      for (int32_t step = kMaxRequests / 2; step > 0; step >>= 1)
+        if (r + step < R && start[r + step] <= u) r += step;
+      const Geometry g = load_request(a, p, r);
+      const int32_t in = u - start[r], parts = cut[r];
+      const int32_t tile = tiles[r] - 1 - in / parts;  // causal tiles: longest first
+      x = int4{r, tile, in % parts, parts};
+      y = int4{record[r] + tile * parts, g.n, g.first, g.len};
+    }
+    list[2 * static_cast<int64_t>(u)] = x;
+    list[2 * static_cast<int64_t>(u) + 1] = y;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    const int32_t head = first_token(a), last = live_tokens(a);
+    list[2 * static_cast<int64_t>(p.units)] = int4{head, last < head ? head : last, 0, 0};
+  }
 }
 
 // ---------------------------------------------------------------- a tile of rows
@@ -525,7 +555,7 @@ __device__ __forceinline__ void wide_tile(const PagedAttnArgs& a, const PagedPas
   const int32_t group = a.group;
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
-  const Work w = find_work<kThreads>(a, p, unit);
+  const Work w = find_work(a, p, unit);
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
@@ -982,7 +1012,7 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   const int32_t group = a.group;
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
-  const Work w = find_work<kThreads>(a, p, unit);
+  const Work w = find_work(a, p, unit);
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
@@ -1521,6 +1551,10 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
     at += round256(rows * 8);
   };
   if (may_cut || l.shared) place(l.own, l.own_units, tiles);
+  if (requests > kPlanned) {
+    l.own.list = reinterpret_cast<const int4*>(static_cast<char*>(workspace) + at);
+    at += round256((2 * l.own_units + 1) * 16);
+  }
   if (l.shared) {
     l.pre = l.own;
     l.pre.shared = 1;
@@ -1550,6 +1584,13 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
   const auto grid = [&](int64_t units) { return dim3(static_cast<uint32_t>(units * a.kv_heads)); };
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
+  if (a.requests > kPlanned) {
+    const int64_t groups = (l.own_units + 4095) / 4096;
+    paged_plan_kernel<<<dim3(static_cast<uint32_t>(groups < 256 ? groups : 256)), 1024, 0, stream>>>(
+        a, l.own, const_cast<int4*>(l.own.list));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   const auto run = [&](const PagedPass& p, Form form, int64_t units) {
     constexpr int kMore = D == 128 ? 1 : 2;  // rows of 64 are half as long
     switch (form) {

@@ -242,3 +242,42 @@ def test_query_starts_out_of_order(device, prefix):
     for starts in ([0, 132, 0, 132], [132, 0, 132, 0], [-5, 9000, 7, -1]):
         fn(**{**a, "query_starts": torch.tensor(starts, dtype=torch.int32, device=device)})
     assert torch.equal(fn(**a), want)
+
+
+@pytest.mark.parametrize("requests,prefix", [(65, 0), (65, 700), (200, 0), (1025, 0), (1500, 90), (4096, 0)])
+def test_many_requests(device, requests, prefix):
+    """More requests than a wave plans: none, one and several tokens each, lengths from 0, one long request."""
+    rng = np.random.default_rng(requests)
+    counts = rng.choice([0, 1, 1, 1, 2, 9], requests)
+    lengths = counts + rng.integers(0, 60, requests)
+    lengths[counts == 0] -= rng.integers(0, 2, int((counts == 0).sum())) * lengths[counts == 0]
+    lengths[requests // 2] += 1500
+    counts[0] = 0
+    b = Batch(lengths, counts, 4, 2, dim=64, prefix=prefix, pad=3)
+    fn = paged_shared_prefix_attention if prefix else paged_window_attention
+    out, l = fn(**b.kwargs(), return_lse=True)
+    b.check(out, l)
+
+
+def test_many_prompts(device):
+    """Several 128-row tiles each, cut and whole, for more requests than a wave plans."""
+    rng = np.random.default_rng(3)
+    counts = rng.integers(30, 130, 70)
+    lengths = counts + rng.integers(0, 40, 70)
+    lengths[[0, 69]] += 900
+    b = Batch(lengths, counts, 8, 2, dim=64, window=200, sinks=5)
+    out, l = paged_window_attention(**b.kwargs(), return_lse=True)
+    b.check(out, l)
+
+
+@pytest.mark.parametrize("prefix", [0, 2500])
+def test_many_query_starts_out_of_order(device, prefix):
+    counts = [2] * 100
+    b = Batch([300] * 100, counts, 8, 2, prefix=prefix)
+    fn = paged_shared_prefix_attention if prefix else paged_window_attention
+    a = b.kwargs()
+    want = fn(**a)
+    up_down = torch.tensor([0, 200], dtype=torch.int32, device=device).repeat(51)[:101].contiguous()
+    for starts in (up_down, 200 - up_down, torch.full_like(up_down, -7), up_down * 10**6):
+        fn(**{**a, "query_starts": starts})
+    assert torch.equal(fn(**a), want)
