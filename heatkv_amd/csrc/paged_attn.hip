@@ -1286,8 +1286,9 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
 }
 
 template <int DT, int D, int NW, int NS>
-__global__ __launch_bounds__(NW * 64, 1) void paged_narrow_kernel(const PagedAttnArgs a, const PagedPass p,
-                                                              const Scalars sc) {
+__global__ __launch_bounds__(NW * 64, NW * NS * D <= 256 ? 2 : 1) void paged_narrow_kernel(const PagedAttnArgs a,
+                                                                                 const PagedPass p,
+                                                                                 const Scalars sc) {
   __shared__ __attribute__((aligned(1024))) NarrowLds<D, NS> lds[NW];
   __shared__ int32_t turn;
   narrow_tile<DT, D, NW, NS>(a, p, sc, static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), lds, turn);
@@ -1427,6 +1428,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnArgs 
 enum Form : int32_t {
   kWide,        // paged_wide_kernel, two workgroups per CU
   kNarrowMany,  // paged_narrow_kernel: two waves of two stages, two workgroups per CU
+  kNarrowMost,  // ... two waves of one stage, four workgroups per CU
   kNarrowOne,   // ... eight waves of one stage, one workgroup per CU
 };
 
@@ -1445,6 +1447,7 @@ int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 int64_t units_bound(const PagedPass& p, int64_t tiles, int64_t chunks) {
   // total / c for any total up to this one: c >= least, and c >= total / wanted or
   // else c >= cap and c >= total / most
+  if (chunks <= p.least || chunks <= p.uncut) return tiles;
   const int64_t total = tiles * chunks;
   int64_t cuts = total / p.cap < p.most ? total / p.cap : p.most;
   if (cuts < p.wanted) cuts = p.wanted;
@@ -1466,7 +1469,10 @@ int64_t units_bound(const PagedPass& p, int64_t tiles, int64_t chunks) {
 // * long tiles: eight waves, in parts of up to 48 chunks (64 requests of up to 16000 rows
 //   418, two waves 436; one of 64000 58 / 68); many short ones: two waves, two workgroups
 //   per CU (256 requests of up to 1200 rows 143, eight waves 160 to 169), whole up to 16
-//   chunks (32 requests of 1000 rows 30.7 / 34.7).
+//   chunks (32 requests of 1000 rows 30.7 / 34.7), and with more than 512 tiles of up to 16
+//   chunks four workgroups of one stage each, so that one's start is hidden by three
+//   others (128 requests of 500 rows 58.0, two 60.5; 1024 of 62 rows 70 / 106; but 64 of
+//   500, 512 tiles, 30.8 / 30.2, and the 256 of up to 1200 140 / 138).
 Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_heads) {
   p.cap = 0x7fffffff;
   p.step = 1;
@@ -1494,7 +1500,8 @@ Form shape(PagedPass& p, bool narrow, int64_t tiles, int64_t chunks, int32_t kv_
   p.cap = 48;
   p.step = one ? 4 : 1;
   p.uncut = one ? 0 : 16;
-  return one ? kNarrowOne : kNarrowMany;
+  if (one) return kNarrowOne;
+  return tiles * kv_heads > 512 && chunks <= 16 ? kNarrowMost : kNarrowMany;
 }
 
 Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_heads, int32_t dim, int64_t table_rows,
@@ -1530,7 +1537,10 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
   l.own.with_prefix = prefix_len > 0 && !l.shared;
   if (l.own.with_prefix) longest += prefix_chunks;
   l.own.always = l.shared;
-  const int64_t tiles = rows / l.own.rows + (busy > 0 ? busy : 1);  // without requests, the tail is filled
+  int64_t tiles = rows / l.own.rows + busy;
+  const int64_t singly = tokens * ((group + l.own.rows - 1) / l.own.rows);  // a request each
+  if (singly < tiles) tiles = singly;
+  if (tiles == 0) tiles = 1;  // without requests, the tail is filled
   l.own_form = shape(l.own, narrow, tiles, longest, kv_heads);
   l.own_units = units_bound(l.own, tiles, longest);
   l.own.units = static_cast<int32_t>(l.own_units < 0x7fffffff ? l.own_units : 0x7fffffff);
@@ -1596,6 +1606,7 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
     switch (form) {
       case kWide: paged_wide_kernel<DT, D><<<grid(units), 256, 0, stream>>>(a, p, sc); break;
       case kNarrowMany: paged_narrow_kernel<DT, D, 2, 2 * kMore><<<grid(units), 128, 0, stream>>>(a, p, sc); break;
+      case kNarrowMost: paged_narrow_kernel<DT, D, 2, kMore><<<grid(units), 128, 0, stream>>>(a, p, sc); break;
       case kNarrowOne: paged_narrow_kernel<DT, D, 8, kMore><<<grid(units), 512, 0, stream>>>(a, p, sc); break;
     }
   };
