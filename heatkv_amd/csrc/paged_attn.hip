@@ -487,7 +487,7 @@ __device__ __forceinline__ void fill_tail(const PagedAttnArgs& a, int32_t head, 
   const int64_t row = static_cast<int64_t>(a.heads) * (a.head_dim / 8);  // 16-byte pieces of a token
   const int64_t gap = live - head;
   uint4* const out = reinterpret_cast<uint4*>(a.out);
-  const int64_t at = static_cast<int64_t>(block) * kThreads + threadIdx.x;
+  const int64_t at = static_cast<int64_t>(block) * kThreads + threadIdx.x % kThreads;
   const int64_t step = static_cast<int64_t>(blocks) * kThreads;
   for (int64_t i = at; i < (a.num_tokens - gap) * row; i += step)
     out[i < head * row ? i : i + gap * row] = uint4{0, 0, 0, 0};
@@ -510,7 +510,7 @@ __device__ __forceinline__ void write_meta(const PagedAttnArgs& a, const PagedPa
                                            int32_t kvh) {
   if (!p.combined || w.part != 0 || kvh != 0) return;
   const int32_t group = a.group;
-  for (int32_t i = threadIdx.x; i < t.rows; i += kThreads)
+  for (int32_t i = threadIdx.x % kThreads; i < t.rows; i += kThreads)
     p.meta[static_cast<int64_t>(t.g.first) * group + t.row0 + i] = int2{w.record, t.parts | i << 16};
 }
 
@@ -989,8 +989,9 @@ struct NarrowLds {
   const uint8_t* rows[2][32];
 };
 
-// Workgroup `block` of `blocks`.
-template <int DT, int D, int NW, int NS>
+// Workgroup `block` of `blocks`, or (PAIR) one of the two in a workgroup of twice the
+// waves: they meet at the one barrier and nowhere else.
+template <int DT, int D, int NW, int NS, bool PAIR = false>
 __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedPass& p, const Scalars& sc,
                                             int32_t block, int32_t blocks, NarrowLds<D, NS> (&lds_waves)[NW],
                                             int32_t& turn) {
@@ -1004,7 +1005,7 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   constexpr int KS = D / 32;               // k-steps of S
   constexpr int DB = D / 16;               // 16-wide blocks of O
   constexpr int kPieces = D / 8;           // 16-byte pieces of a row
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x % kThreads;
   const int lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int q = lane & 15;
@@ -1012,11 +1013,18 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   const int32_t group = a.group;
   const int32_t unit = block / a.kv_heads;
   const int32_t kvh = block - unit * a.kv_heads;
+  if (PAIR && block >= blocks) {
+    __syncthreads();
+    return;
+  }
   const Work w = find_work(a, p, unit);
   if (a.fill_tail && !p.shared && w.end - w.head < a.num_tokens)
     fill_tail<kThreads>(a, w.head, w.end, block, blocks);
   Tile t;
-  if (w.request < 0 || !make_tile(a, p, w, unit, t)) return;
+  if (w.request < 0 || !make_tile(a, p, w, unit, t)) {
+    if constexpr (PAIR) __syncthreads();
+    return;
+  }
   write_meta<kThreads>(a, p, t, w, kvh);
 
   const int32_t mat = t.row0 + (q < t.rows ? q : t.rows - 1);
@@ -1253,7 +1261,7 @@ __device__ __forceinline__ void narrow_tile(const PagedAttnArgs& a, const PagedP
   }
   if (t.parts > 1 || p.always) {
     float* const rec = record_of<D>(a, p, w.record + w.part, kvh);
-    const bool join = t.parts > 1 && p.join;
+    const bool join = !PAIR && t.parts > 1 && p.join;
     if (q < t.rows) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
@@ -1301,8 +1309,9 @@ __global__ __launch_bounds__(NW * 64, NW * NS * D <= 256 ? 2 : 1) void paged_nar
 // to the 8 XCDs in turn and to an XCD's 32 CUs in turn, twice: the kinds alternate
 // from CU to CU, and the other way round for a CU's second workgroup.  128 tokens
 // behind 16384 rows, 32 heads on 8: 88.9 us with the combine, 104.2 in two launches (51
-// and 43, and 11); 16 tokens behind 2000 rows, 16 heads: 18.8 / 25.2.
-template <int DT, int D, bool WIDE>
+// and 43, and 11); 16 tokens behind 2000 rows, 16 heads: 18.8 / 25.2.  With more own
+// tiles than CUs a workgroup runs two of them, on two waves each.
+template <int DT, int D, bool WIDE, bool PAIR>
 __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a, const PagedPass pre,
                                                               const PagedPass own, const Scalars sc,
                                                               const int32_t pre_blocks, const int32_t own_blocks) {
@@ -1331,6 +1340,10 @@ __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArg
     if constexpr (WIDE) wide_tile<DT, D>(a, pre, sc, id, pre_blocks, *reinterpret_cast<WideLds<D>*>(lds));
     else
       narrow_tile<DT, D, NW, NS>(a, pre, sc, id, pre_blocks, *reinterpret_cast<NarrowLds<D, NS>(*)[NW]>(lds), turn);
+  } else if constexpr (PAIR) {
+    const int half = uniform(threadIdx.x >> 7);
+    narrow_tile<DT, D, 2, NS, true>(a, own, sc, 2 * id + half, own.units * a.kv_heads,
+                                    reinterpret_cast<NarrowLds<D, NS>(*)[2]>(lds)[half], turn);
   } else {
     narrow_tile<DT, D, NW, NS>(a, own, sc, id, own_blocks, *reinterpret_cast<NarrowLds<D, NS>(*)[NW]>(lds), turn);
   }
@@ -1434,6 +1447,7 @@ enum Form : int32_t {
 
 struct Layout {
   int32_t shared;    // a pass of its own for the prefix ...
+  int32_t pairs;     // ... two of a request's own tiles to a workgroup
   int32_t together;  // ... in one launch with narrow tiles of the requests' own rows
   Form own_form, pre_form;
   PagedPass own, pre;
@@ -1577,6 +1591,8 @@ Layout layout_of(int32_t tokens, int32_t requests, int32_t heads, int32_t kv_hea
       // one per CU beside the requests' own tiles (two: 100 against 88.9 us above)
       l.pre.wanted = l.pre.most = (256 + kv_heads - 1) / kv_heads;
       l.pre.cap = 0x7fffffff;
+      // us, one tile / two to a workgroup: 256 tiles 31.0 / 31.1, 384 26.9 / 23.3, 2048 103 / 95
+      l.pairs = l.own_units * kv_heads > 256;
     }
     l.pre_units = units_bound(l.pre, tiles, prefix_chunks);
     l.pre.units = static_cast<int32_t>(l.pre_units < 0x7fffffff ? l.pre_units : 0x7fffffff);
@@ -1611,12 +1627,17 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
     }
   };
   if (l.together) {
-    const int64_t pre = l.pre_units * a.kv_heads, own = l.own_units * a.kv_heads;
+    const int64_t pre = l.pre_units * a.kv_heads;
+    const int64_t own = l.pairs ? (l.own_units * a.kv_heads + 1) / 2 : l.own_units * a.kv_heads;
     if (pre + own > 0x7fffffffLL / 256) return hipErrorInvalidConfiguration;
     const dim3 all(static_cast<uint32_t>(pre + own));
     const int32_t p = static_cast<int32_t>(pre), o = static_cast<int32_t>(own);
-    if (l.pre_form == kWide) paged_prefix_kernel<DT, D, true><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
-    else paged_prefix_kernel<DT, D, false><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
+    if (l.pre_form == kWide && l.pairs)
+      paged_prefix_kernel<DT, D, true, true><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
+    else if (l.pre_form == kWide)
+      paged_prefix_kernel<DT, D, true, false><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
+    else
+      paged_prefix_kernel<DT, D, false, false><<<all, 256, 0, stream>>>(a, l.pre, l.own, sc, p, o);
   } else {
     if (l.shared) run(l.pre, l.pre_form, l.pre_units);
     run(l.own, l.own_form, l.own_units);

@@ -281,3 +281,16 @@ def test_many_query_starts_out_of_order(device, prefix):
     for starts in (up_down, 200 - up_down, torch.full_like(up_down, -7), up_down * 10**6):
         fn(**{**a, "query_starts": starts})
     assert torch.equal(fn(**a), want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("requests", [95, 131])
+def test_prefix_with_many_tiles(device, requests, dim):
+    """More of the requests' own tiles than CUs beside a prefix in 128-row tiles; an odd number of them."""
+    rng = np.random.default_rng(requests)
+    counts = rng.choice([0, 1, 1, 1, 2, 7], requests)
+    lengths = counts + rng.integers(0, 200, requests)
+    lengths[-1] += 1200
+    b = Batch(lengths, counts, 6, 3, dim=dim, prefix=1500, pad=5)
+    out, l = paged_shared_prefix_attention(**b.kwargs(), return_lse=True)
+    b.check(out, l)
