@@ -13,12 +13,14 @@
 //    requests of 800 to 16000 rows, 2.33 GB: 404 us, 5.8 TB/s; a copy of 2 GiB
 //    moves 4.95.
 //
-// Plan.  Nothing about the requests is known on the host, so every workgroup
-// finds its work from lengths and query_starts itself (1 to 2 us, beside other
-// workgroups' work in all but the smallest launches; a plan made by a launch of its
-// own would cost every call that much): tiles of rows per
-// request, 64-key chunks per tile, and, so that few rows over long keys still
-// fill the card, parts of a tile's chunks.  part_chunks gives the chunks of a
+// Plan.  Nothing about the requests is known on the host, so up to 64 requests every
+// wave finds its work from lengths and query_starts itself (1 to 2 us, beside other
+// workgroups' work in all but the smallest launches); for more, paged_plan_kernel
+// writes each unit's work first, about 4 us (planned by every workgroup: 128 requests of
+// 500 rows 65.4 us against 59.4, 1024 of 62 rows 283 against 106; two requests to a lane
+// would save 3 us up to 128 requests and cost the calls of a few 0.2).  The plan is tiles
+// of rows per request, 64-key chunks per tile, and, so that few rows over long keys
+// still fill the card, parts of a tile's chunks.  part_chunks gives the chunks of a
 // part from the total of the launch, so that the host knows how many units and
 // records there can be at most.  A tile that is not cut writes its output.  Parts of
 // narrow tiles are joined by the last of them (join_parts): a pair of tokens over
@@ -217,8 +219,8 @@ __device__ __forceinline__ int2 wave_prefix(int2 v, int n = 64) {
   return v;
 }
 
-// Work of unit `unit` (per K/V head).  Up to 64 requests every wave plans by
-// itself, a request per lane; more are dealt to the workgroup's threads in runs.
+// Work of unit `unit` (per K/V head): up to kPlanned requests every wave plans by
+// itself, a request per lane.
 __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPass& p, int32_t unit) {
   const int32_t R = p.shared ? 1 : a.requests;
   const int lane = threadIdx.x & 63;
