@@ -233,3 +233,30 @@ def test_unaligned_cache_is_refused(device):
     c = torch.zeros(a["k_cache"].numel() + 1, dtype=torch.bfloat16, device=device)[1:].view_as(a["k_cache"])
     with pytest.raises(ValueError, match="16-byte"):
         paged_window_attention(**{**a, "k_cache": c})
+
+
+@pytest.mark.parametrize("prefix", [0, 1500])
+def test_captured_with_many_requests(device, prefix):
+    """More requests than a wave plans: a graph follows lengths and starts that change between replays."""
+    n = 150
+    rng = np.random.default_rng(5)
+    counts = np.ones(n, np.int64)
+    b = Batch(rng.integers(100, 400, n), counts, 8, 2, prefix=prefix)
+    a = b.kwargs()
+    a["k_cache"], a["v_cache"] = (torch.nan_to_num(a[x]) for x in ("k_cache", "v_cache"))
+    fn = paged_shared_prefix_attention if prefix else paged_window_attention
+    fn(**a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn(**a)
+    for i in range(4):
+        keep = rng.integers(0, 3, n)  # tokens of each request, as many of them as there is room for
+        starts = np.minimum(np.concatenate([[0], np.cumsum(keep)]), n).astype(np.int32)
+        a["query_starts"].copy_(torch.from_numpy(starts))
+        a["lengths"].copy_(torch.from_numpy(rng.integers(2, 100, n).astype(np.int32)))
+        want = fn(**a)
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert torch.equal(out, want)
