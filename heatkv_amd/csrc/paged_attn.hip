@@ -16,7 +16,7 @@
 // Plan.  Nothing about the requests is known on the host, so up to 64 requests every
 // wave finds its work from lengths and query_starts itself (1 to 2 us, beside other
 // workgroups' work in all but the smallest launches); for more, paged_plan_kernel
-// writes each unit's work first, about 4 us (planned by every workgroup: 128 requests of
+// writes each unit's work first, about 5 us (planned by every workgroup: 128 requests of
 // 500 rows 65.4 us against 59.4, 1024 of 62 rows 283 against 106; two requests to a lane
 // would save 3 us up to 128 requests and cost the calls of a few 0.2).  The plan is tiles
 // of rows per request, 64-key chunks per tile, and, so that few rows over long keys
@@ -270,14 +270,16 @@ __device__ __forceinline__ Work find_work(const PagedAttnArgs& a, const PagedPas
 }
 
 // The work of every unit of a launch of more than kPlanned requests, 32 bytes each, and
-// behind them the range of live tokens.  Each workgroup plans all requests, four to a
-// thread, and finds its own units' requests by bisection.
-__global__ __launch_bounds__(1024) void paged_plan_kernel(const PagedAttnArgs a, const PagedPass p,
-                                                          int4* __restrict__ list) {
-  constexpr int kThreads = 1024, kWaves = kThreads / 64, kRun = kMaxRequests / kThreads;
+// behind them the range of live tokens.  Each workgroup plans all requests, up to four
+// to a thread, and finds its own units' requests by bisection.  256 threads up to 1024
+// requests: 128 requests of 500 rows 56.6 us, with 1024 threads 57.7.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void paged_plan_kernel(const PagedAttnArgs a, const PagedPass p,
+                                                              int4* __restrict__ list) {
+  constexpr int kWaves = kThreads / 64, kRun = kMaxRequests / 1024, kMost = kThreads * kRun;
   __shared__ int64_t wave_total[kWaves];
   __shared__ int2 wave_units[kWaves];
-  __shared__ int32_t start[kMaxRequests], record[kMaxRequests], tiles[kMaxRequests], cut[kMaxRequests];
+  __shared__ int32_t start[kMost], record[kMost], tiles[kMost], cut[kMost];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = tid >> 6;
@@ -325,7 +327,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(const PagedAttnArgs a,
     int4 x{-1, 0, 0, 1}, y{0, 0, 0, 0};
     if (u < all.x) {
       int32_t r = 0;  // the last request that starts at or before u
-      for (int32_t step = kMaxRequests / 2; step > 0; step >>= 1)
+      for (int32_t step = kMost / 2; step > 0; step >>= 1)
         if (r + step < R && start[r + step] <= u) r += step;
       const Geometry g = load_request(a, p, r);
       const int32_t in = u - start[r], parts = cut[r];
@@ -1613,9 +1615,12 @@ hipError_t launch(const PagedAttnArgs& a, const Scalars& sc, hipStream_t stream)
   if ((l.own_units > l.pre_units ? l.own_units : l.pre_units) * a.kv_heads > 0x7fffffffLL / 256)
     return hipErrorInvalidConfiguration;
   if (a.requests > kPlanned) {
-    const int64_t groups = (l.own_units + 4095) / 4096;
-    paged_plan_kernel<<<dim3(static_cast<uint32_t>(groups < 256 ? groups : 256)), 1024, 0, stream>>>(
-        a, l.own, const_cast<int4*>(l.own.list));
+    const bool few = a.requests <= 1024;
+    const int64_t groups = few ? (l.own_units + 255) / 256 : (l.own_units + 4095) / 4096;
+    const dim3 plan(static_cast<uint32_t>(groups < 256 ? groups : 256));
+    int4* const list = const_cast<int4*>(l.own.list);
+    if (few) paged_plan_kernel<256><<<plan, 256, 0, stream>>>(a, l.own, list);
+    else paged_plan_kernel<1024><<<plan, 1024, 0, stream>>>(a, l.own, list);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

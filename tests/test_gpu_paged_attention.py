@@ -244,7 +244,7 @@ def test_query_starts_out_of_order(device, prefix):
     assert torch.equal(fn(**a), want)
 
 
-@pytest.mark.parametrize("requests,prefix", [(65, 0), (65, 700), (200, 0), (1025, 0), (1500, 90), (4096, 0)])
+@pytest.mark.parametrize("requests,prefix", [(65, 0), (65, 700), (200, 0), (1024, 0), (1025, 0), (1500, 90), (4096, 0)])
 def test_many_requests(device, requests, prefix):
     """More requests than a wave plans: none, one and several tokens each, lengths from 0, one long request."""
     rng = np.random.default_rng(requests)
