@@ -1314,7 +1314,8 @@ __global__ __launch_bounds__(NW * 64, NW * NS * D <= 256 ? 2 : 1) void paged_nar
 // from CU to CU, and the other way round for a CU's second workgroup.  128 tokens
 // behind 16384 rows, 32 heads on 8: 88.9 us with the combine, 104.2 in two launches (51
 // and 43, and 11); 16 tokens behind 2000 rows, 16 heads: 18.8 / 25.2.  With more own
-// tiles than CUs a workgroup runs two of them, on two waves each.
+// tiles than CUs a workgroup runs two of them, on two waves each (the 128 tokens 69 us of
+// this kernel against 79, part of that by the plan launch).
 template <int DT, int D, bool WIDE, bool PAIR>
 __global__ __launch_bounds__(256, 2) void paged_prefix_kernel(const PagedAttnArgs a, const PagedPass pre,
                                                               const PagedPass own, const Scalars sc,
